@@ -637,6 +637,64 @@ int sg_sample_fix_neighbor_hip(int32_t* sampled, int32_t* dst_ind_ptr, const int
                                const int32_t* sel_indices, int64_t sel_num, int64_t neighbor_num, uint64_t seed,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * (13) the catalogue head: a row's answer out of the whole item catalogue, and the loss that trains it.  No reference
+ *      counterpart (the reference scores given pairs only).  Rows are row-major with a pitch in elements; float types are
+ *      SG_DTYPE_*.  Nothing here needs zeroed or kept memory: a call may be captured into a graph and replayed.
+ * ---------------------------------------------------------------------------------------------- */
+#define SG_DTYPE_F32 0
+#define SG_DTYPE_F16 1
+#define SG_DTYPE_BF16 2
+
+/* Rows as 8-bit codes with one scale a row, behind an optional root-mean-square norm with the residual's addition:
+ *   h = x (+ residual), rounded to the rows' type;  y = h / sqrt(mean(h^2) + eps) * weight (norm != 0), else y = h * weight
+ *   scale = max|y| / 127 (fp32),  code = rint(y / scale), ties to even, in [-127, 127]
+ * residual, weight (NULL: ones) and sum (receives h; may be x or residual themselves) may be NULL.  weight has the rows' type,
+ * or fp32 where weight_f32 != 0.  codes (rows, dim), scale (rows) and sum (rows, dim) are contiguous.  A row that is not
+ * finite, or whose scale is not, has scale NaN and codes 0; a row of zeros scale 0.  1 <= dim <= SG_QUANT_ROWS_MAX_DIM. */
+#define SG_QUANT_ROWS_MAX_DIM 16384
+int sg_quant_rows_i8_hip(int8_t* codes, float* scale, void* sum, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                         const void* weight, int weight_f32, int64_t rows, int64_t dim, int dtype, int norm, double eps,
+                         void* stream);
+
+/* C[m, n] = act(sa[m] * sb[n] * sum_k A[m, k] B[n, k] + bias[n]): A (M, K), B (N, K) 8-bit codes, exact 32-bit sums
+ * (K < SG_GEMM_I8_MAX_K), C of type `dtype`; bias may be NULL.  Any alignment and pitch; 16-byte aligned operands with
+ * pitches that are multiples of 16 are faster.  K = 0 gives act(bias). */
+#define SG_GEMM_I8_MAX_K 131072
+size_t sg_gemm_i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int sg_gemm_i8_hip(void* C, int64_t ldc, int dtype, const int8_t* A, int64_t lda, const float* sa, const int8_t* B, int64_t ldb,
+                   const float* sb, const float* bias, int64_t M, int64_t N, int64_t K, int act, float slope, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* One item a row from its scores.  w_i = exp((l_i - max l) / temperature); the order of a row: larger score first, lower index
+ * first among equals; kept: the shortest prefix of the order that leaves top_k items (0: all), the first items that hold the
+ * share top_p of the top-k items' weight (>= 1: all) and items with w_i >= min_p, but at least the first item.  ids[row] = the
+ * first index at which the kept weight up to it exceeds u[row] times the kept weight, prob[row] = its share.  temperature 0,
+ * top_p 0 or min_p > 1 leave the first item.  Scores of -inf and NaN are never drawn; a row of nothing else gets -1 and 0.
+ * Settings are scalars, or one a row where the *_rows pointer is not NULL (values below 0 count as 0 there).  u in [0, 1). */
+#define SG_SAMPLE_MAX_ITEMS (1 << 30)
+size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n);
+int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld, int dtype, const float* u, int64_t rows, int64_t n,
+                       double temperature, int64_t top_k, double top_p, double min_p, const float* temperature_rows,
+                       const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* A student's scores fitted to a teacher's top scores.  q = softmax(student / temperature) over the n items of a row, p =
+ * softmax(teacher / temperature) over its k entries (item ids):
+ *   loss = scale * temperature^2 * sum_rows sum_k p_k (log p_k - log q_{ids_k})
+ *   grad = grad_loss * scale * temperature * (q - p)
+ * An id outside [0, n) or a teacher score of -inf is no entry; a row without an entry, or without a student score above -inf,
+ * adds no loss and gets a zero gradient.  An item may be named more than once.  The forward leaves stats (rows, 2) and p
+ * (rows, k) for the backward; grad (rows, n) is contiguous and of the student's type; grad_loss is one number on the device. */
+#define SG_DISTILL_MAX_K 1024
+size_t sg_distill_workspace_bytes(int64_t rows, int64_t n);
+int sg_distill_hip(float* loss, float* stats, float* p, const void* student, int64_t ld, int dtype, const float* teacher,
+                   const int32_t* ids, int64_t rows, int64_t n, int64_t k, float temperature, float scale, void* workspace,
+                   size_t workspace_bytes, void* stream);
+int sg_distill_bwd_hip(void* grad, const void* student, int64_t ld, int dtype, const float* stats, const float* p,
+                       const int32_t* ids, int64_t rows, int64_t n, int64_t k, float temperature, float scale,
+                       const float* grad_loss, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

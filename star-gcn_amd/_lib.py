@@ -16,6 +16,7 @@ SO_PATH = os.environ.get("SG_LIB_OVERRIDE") or os.path.join(CSRC, "libstargcn_hi
 
 REQ_NULL, REQ_WRITE, REQ_ADD = 0, 1, 3
 POOL = {"sum": 0, "avg": 1, "max": 2}
+DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # SG_DTYPE_*
 ACT = {None: 0, "identity": 0, "none": 0, "leaky": 1, "relu": 2, "sigmoid": 3, "tanh": 4}
 
 
@@ -33,7 +34,7 @@ def build(force=False, verbose=False):
 
 
 _c = ctypes
-_P, _I64, _INT, _F32, _SZ = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_size_t
+_P, _I64, _INT, _F32, _F64, _SZ = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_double, _c.c_size_t
 
 # name -> (restype, argtypes)   -- kept in the order of include/stargcn.h
 _SIGS = {
@@ -149,6 +150,14 @@ _SIGS = {
                                  _c.c_int32, _I64, _I64, _I64, _INT, _INT, _F32, _INT, _P, _SZ, _P]),
     "sg_agg_fused_profile_enable": (_INT, [_INT]),
     "sg_agg_fused_profile_read": (_I64, [_P, _P, _P, _I64]),
+    "sg_quant_rows_i8_hip": (_INT, [_P] * 4 + [_I64, _P, _I64, _P, _INT, _I64, _I64, _INT, _INT, _F64, _P]),
+    "sg_gemm_i8_workspace_bytes": (_SZ, [_I64] * 3),
+    "sg_gemm_i8_hip": (_INT, [_P, _I64, _INT, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _INT, _F32, _P, _SZ, _P]),
+    "sg_sample_rows_workspace_bytes": (_SZ, [_I64] * 2),
+    "sg_sample_rows_hip": (_INT, [_P, _P, _P, _I64, _INT, _P, _I64, _I64, _F64, _I64, _F64, _F64] + [_P] * 5 + [_SZ, _P]),
+    "sg_distill_workspace_bytes": (_SZ, [_I64] * 2),
+    "sg_distill_hip": (_INT, [_P] * 4 + [_I64, _INT, _P, _P, _I64, _I64, _I64, _F32, _F32, _P, _SZ, _P]),
+    "sg_distill_bwd_hip": (_INT, [_P, _P, _I64, _INT, _P, _P, _P, _I64, _I64, _I64, _F32, _F32, _P, _P]),
 }
 
 
@@ -210,6 +219,21 @@ def require_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise StarGCNError("expected a CUDA/HIP tensor, got a %s tensor" % t.device)
+
+
+def require_current_gpu(*tensors):
+    """require_gpu, and that every tensor lives on the current device: kernels go to that device's current stream."""
+    require_gpu(*tensors)
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise StarGCNError("a tensor is on %s but the current device is cuda:%d (torch.cuda.device selects it)" % (t.device, cur))
+
+
+def scratch(nbytes, device):
+    """A call's own scratch memory from torch's allocator: ordered with the current stream, and part of the graph's own pool
+    while one is captured, so that no two graphs share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def ptr(t):

@@ -1,0 +1,158 @@
+// quant_rows.hip -- rows to 8-bit codes with one scale a row, optionally behind a root-mean-square norm with the residual's
+// addition: what feeds the 8-bit product (gemm_i8.hip).
+//
+//   h = rnd(x + residual)      rounded to the type of x: the stored sum, and what everything below reads
+//   y = h / sqrt(mean(h^2) + eps) * w              (norm)          y = h           (no norm)
+//   scale = fl32(max|y| / 127),   code = rint(y / scale) in [-127, 127], ties to even
+//
+// A code is a decision at the border between two whole numbers, so everything up to it is held in 64 bits: the sum of
+// squares, y (an fp32 h times an fp32 w is exact in 64 bits) and the quotient.  The card's 64-bit vector rate makes that
+// cheap: ~10 operations an element against 7..13 bytes of memory traffic.  A row with an infinity or a NaN in it, or whose
+// scale overflows 32 bits, has no codes: scale NaN, codes 0, so that a product with it is NaN.  A row of zeros has scale 0.
+//
+// Memory bound: x and the residual are read once, codes and the sum written once; a row stays in the registers of its
+// threads between its reduction and its codes.
+#include "common.hpp"
+#include "rows_shared.hpp"
+
+namespace sg {
+namespace {
+
+struct QuantArgs {
+  int8_t* codes;
+  float* scale;
+  void* sum;
+  const void* x;
+  const void* res;
+  const void* w;
+  long long ldx, ldr;
+  long long rows;
+  int dim, norm, w_f32;
+  double eps;
+};
+
+// TPR threads a row, NV 16-byte vectors a thread
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quant_rows_kernel(const QuantArgs g) {
+  constexpr int V = 16 / sizeof(T), THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR, WPR = TPR / kWave;
+  __shared__ double red[2][THREADS / kWave];
+  const int t = threadIdx.x % TPR;
+  const long long row = static_cast<long long>(blockIdx.x) * RPB + threadIdx.x / TPR;
+  const bool live = row < g.rows;
+  const T* x = static_cast<const T*>(g.x) + row * g.ldx;
+  const T* res = g.res ? static_cast<const T*>(g.res) + row * g.ldr : nullptr;
+  T* sum = g.sum ? static_cast<T*>(g.sum) + row * g.dim : nullptr;
+  double p[NV][V];                                       // h * w, exact
+  double ss = 0.0, top = 0.0, bad = 0.0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * V, n = live ? min(V, g.dim - c) : 0;
+    float h[V], r[V], w[V];
+    load_vec<T, V>(h, x + c, n);
+    if (res) {
+      load_vec<T, V>(r, res + c, n);
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[j] = round_to<T>(h[j] + r[j]);
+    }
+    if (sum) store_vec<T, V>(sum + c, h, n);
+    if (!g.w) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = 1.f;
+    } else if (g.w_f32) {
+      load_vec<float, V>(w, static_cast<const float*>(g.w) + c, n);
+    } else {
+      load_vec<T, V>(w, static_cast<const T*>(g.w) + c, n);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (j >= n) h[j] = 0.f, w[j] = 0.f;
+      const double hd = h[j];
+      p[i][j] = hd * static_cast<double>(w[j]);
+      if (g.norm) ss = fma(hd, hd, ss);
+      top = fmax(top, fabs(p[i][j]));
+      bad = fma(p[i][j], 0.0, bad);                      // NaN once a value is not finite (fmax drops NaNs)
+    }
+  }
+  ss += bad;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    ss += __shfl_xor(ss, off);
+    top = fmax(top, __shfl_xor(top, off));
+  }
+  if (WPR > 1) {
+    const int wave = threadIdx.x / kWave;
+    if (threadIdx.x % kWave == 0) red[0][wave] = ss, red[1][wave] = top;
+    __syncthreads();
+    ss = 0.0, top = 0.0;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) ss += red[0][i], top = fmax(top, red[1][i]);
+  }
+  if (!live) return;
+  const double rstd = g.norm ? 1.0 / sqrt(ss / g.dim + g.eps) : 1.0 + ss * 0.0;
+  float scale = static_cast<float>(top * rstd / 127.0);
+  const bool none = !(scale <= 3.402823466e38f) || !(rstd <= 1.7976931348623157e308);      // NaN and infinities
+  if (none) scale = __builtin_nanf("");
+  if (t == 0) g.scale[row] = scale;
+  const double s = scale, inv = (none || scale == 0.f) ? 0.0 : 1.0 / s;
+  int8_t* codes = g.codes + row * g.dim;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * V, n = min(V, g.dim - c);
+    int q[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double y = none ? 0.0 : p[i][j] * rstd, a = y * inv;
+      double k = rint(a);
+      if (fabs(fabs(a - k) - 0.5) < 1e-6) {              // near a tie: decide by the exact remainder, not the reciprocal
+        const double r = fma(-k, s, y), far = 2.0 * fabs(r) - s;
+        const bool odd = (static_cast<int>(k) & 1) != 0;
+        if (far > 0.0 || (far == 0.0 && odd)) k += copysign(1.0, r);
+      }
+      q[j] = static_cast<int>(fmin(fmax(k, -127.0), 127.0));
+    }
+    store_codes<V>(codes + c, q, n);
+  }
+}
+
+template <typename T, int TPR, int NV>
+void launch(const QuantArgs& g, hipStream_t st) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPB = THREADS / TPR;
+  hipLaunchKernelGGL((quant_rows_kernel<T, TPR, NV>), dim3(static_cast<unsigned>((g.rows + RPB - 1) / RPB)), dim3(THREADS), 0, st, g);
+}
+
+// the narrowest form that holds a row: a wave for short rows (no barrier, four rows a workgroup), else a workgroup
+template <typename T>
+void dispatch(const QuantArgs& g, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const int vecs = (g.dim + V - 1) / V;
+  if (vecs <= 64) launch<T, 64, 1>(g, st);
+  else if (vecs <= 128) launch<T, 64, 2>(g, st);
+  else if (vecs <= 256) launch<T, 256, 1>(g, st);
+  else if (vecs <= 512) launch<T, 256, 2>(g, st);
+  else if (vecs <= 1024) launch<T, 256, 4>(g, st);
+  else if (vecs <= 2048) launch<T, 1024, 2>(g, st);
+  else launch<T, 1024, 4>(g, st);
+}
+
+}  // namespace
+}  // namespace sg
+
+using namespace sg;
+
+SG_API int sg_quant_rows_i8_hip(int8_t* codes, float* scale, void* sum, const void* x, int64_t ldx, const void* residual,
+                                int64_t ldr, const void* weight, int weight_f32, int64_t rows, int64_t dim, int dtype, int norm,
+                                double eps, void* stream) {
+  if (!valid_dtype(dtype)) return fail(SG_ERR_INVALID, "quant_rows: unknown dtype %d", dtype);
+  if (rows < 0 || dim < 1 || rows >= (1ll << 31)) return fail(SG_ERR_INVALID, "quant_rows: bad shape");
+  if (dim > SG_QUANT_ROWS_MAX_DIM) return fail(SG_ERR_UNSUPPORTED, "quant_rows: rows of at most %d elements", SG_QUANT_ROWS_MAX_DIM);
+  if (norm && !(eps >= 0.0)) return fail(SG_ERR_INVALID, "quant_rows: eps must not be negative");
+  if (rows == 0) return SG_OK;
+  if (!codes || !scale || !x) return fail(SG_ERR_INVALID, "quant_rows: null pointer argument");
+  if (ldx < dim || (residual && ldr < dim)) return fail(SG_ERR_INVALID, "quant_rows: rows overlap");
+  QuantArgs g{codes, scale, sum, x, residual, weight, ldx, ldr, rows, static_cast<int>(dim), norm, weight_f32, eps};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == SG_DTYPE_F32) dispatch<float>(g, st);
+  else if (dtype == SG_DTYPE_F16) dispatch<f16>(g, st);
+  else dispatch<bf16>(g, st);
+  return check_launch("quant_rows");
+}

@@ -5,6 +5,7 @@
                      (sg_multilink_agg_fwd_hip: one gather launch + one MFMA contraction; the reference runs
                      R FullyConnected + R seg_weighted_pool + add_n/concat + activation)
   take_rows / masked_embed   row gathers with atomic-free, plan-based gradients
+  distill_loss       a student's scores over the item catalogue fitted to a teacher's top scores
 
 Association order of the aggregation.  The reference computes  A_r (X W_r^T + 1 b_r^T)  ("transform first").
 Algebraically that equals  (A_r X) W_r^T + (A_r 1) b_r^T  ("aggregate first").  Either way ONE side of the
@@ -167,3 +168,27 @@ def l2_loss(pred, target, scale):
     """scale * sum 0.5 (pred - target)^2 -- gluon L2Loss of the reference (STAR-GCN.py:550,612) with the reduction;
     value and gradient come from one native pass (sg_l2_loss_hip).  `target` gets no gradient."""
     return _L2Loss.apply(pred, target, scale)
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, student, teacher, ids, scale, temperature):
+        ids = L.i32c(ids)
+        loss, stats, p = ops.distill_fwd(student, teacher, ids, scale, temperature)
+        ctx.scale, ctx.temperature = scale, temperature
+        ctx.save_for_backward(student, ids, stats, p)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        student, ids, stats, p = ctx.saved_tensors
+        return ops.distill_bwd(g, student, stats, p, ids, ctx.scale, ctx.temperature), None, None, None, None
+
+
+def distill_loss(student, teacher, ids, scale, temperature=1.0):
+    """scale * temperature^2 * sum over rows of KL(p || q): p = softmax(teacher / temperature) over the teacher's k best items of
+    a row, q = softmax(student / temperature) over all its items.  student (rows, items) fp32 / fp16 / bf16 scores, teacher
+    (rows, k) their scores, ids (rows, k) their items.  An id outside the items (-1) or a teacher score of -inf is padding; a row
+    of padding, or with no student score above -inf, adds nothing.  The teacher gets no gradient."""
+    return _Distill.apply(student, teacher, ids, float(scale), float(temperature))

@@ -417,14 +417,9 @@ class Net(nn.Module):
         return plan
 
     # ---- device work (reference STAR-GCN.py:399-461) --------------------------------------------------
-    def run(self, plan, rating_targets=None, rating_scale=None):
-        """rating_targets (standardised ratings of the plan's pairs) + rating_scale: return per-block rating LOSSES
-        scale * sum 0.5 (score - y)^2 in place of the scores (fused rating head, sg_pair_l2_hip) -- what training needs;
-        evaluation keeps the scores."""
-        pred_ratings, pred_embeddings = [], []
-        gt = self.get_embed(plan["gt"]) if plan["gt"] is not None else dict()
-        if gt and self._recon_fea:
-            gt = self._concat(gt, self.get_feature(plan["gt_fea"]))
+    def _encode(self, plan):
+        """(k, index plans, encoder output) of every block in turn, k = the block's parameters; the decoder that feeds the next
+        block runs when the caller asks for it."""
         x = self.get_embed(plan["input"]) if self._use_embed else None
         if self._use_fea_proj:      # STAR-GCN.py:405-413
             fea = self.get_feature(plan["input_fea"])
@@ -434,6 +429,22 @@ class Net(nn.Module):
             out = enc.heter_sage(x, plan["enc"][b])
             idx = plan["idx"][b]
             k = 0 if self._use_recurrent else b
+            yield k, idx, out
+            if b < self._nblocks - 1 and self._use_dae:
+                m = self.embed_maps[k]
+                x = {key: m[key](SF.take_rows(out[key], tp)) for key, tp in idx["req_take"].items()}
+                if "req_fea" in idx:
+                    x = self._concat(x, self.get_feature(idx["req_fea"]))
+
+    def run(self, plan, rating_targets=None, rating_scale=None):
+        """rating_targets (standardised ratings of the plan's pairs) + rating_scale: return per-block rating LOSSES
+        scale * sum 0.5 (score - y)^2 in place of the scores (fused rating head, sg_pair_l2_hip) -- what training needs;
+        evaluation keeps the scores."""
+        pred_ratings, pred_embeddings = [], []
+        gt = self.get_embed(plan["gt"]) if plan["gt"] is not None else dict()
+        if gt and self._recon_fea:
+            gt = self._concat(gt, self.get_feature(plan["gt_fea"]))
+        for k, idx, out in self._encode(plan):
             if "pair" in idx:   # Dense is row-wise, so project the unique rows first, then pair them up
                 pu = self.rating_user_projs[k](out[self._name_user])
                 pi = self.rating_item_projs[k](out[self._name_item])
@@ -453,12 +464,14 @@ class Net(nn.Module):
                 m = self.embed_maps[k]
                 pred_embeddings.append({key: m[key](SF.take_rows(out[key], tp))
                                         for key, tp in idx["recon_take"].items()})
-            if b < self._nblocks - 1 and self._use_dae:
-                m = self.embed_maps[k]
-                x = {key: m[key](SF.take_rows(out[key], tp)) for key, tp in idx["req_take"].items()}
-                if "req_fea" in idx:
-                    x = self._concat(x, self.get_feature(idx["req_fea"]))
         return pred_ratings, pred_embeddings, gt
+
+    def rating_rows(self, plan):
+        """(user rows, item rows) of the last block's rating projections, one row a node that the plan computes there: a pair's
+        score is the inner product of its two rows.  What a CatalogueHead (star_gcn_amd.recommend) is made of and asked with."""
+        for k, _idx, out in self._encode(plan):
+            pass
+        return self.rating_user_projs[k](out[self._name_user]), self.rating_item_projs[k](out[self._name_item])
 
     def forward(self, graph, rating_node_pairs=None, embed_noise_dict=None, recon_node_ids_dict=None,
                 graph_sampler_args=None, symm=None, device="cuda", rating_targets=None, rating_scale=None):

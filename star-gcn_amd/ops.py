@@ -437,3 +437,166 @@ def l2_loss_fwd(pred, target, scale):
     L.check(lib.sg_l2_loss_hip(L.ptr(loss), L.ptr(grad), L.ptr(pred), L.ptr(target), n, float(scale), L.ptr(ws), wsn,
                                L.stream_ptr()), "sg_l2_loss_hip")
     return loss, grad
+
+
+# ---- the catalogue head -----------------------------------------------------------------------------------------------
+
+
+def _dtype_id(t, what):
+    if t.dtype not in L.DTYPE:
+        raise L.StarGCNError("%s: float32, float16 or bfloat16 expected, got %s" % (what, t.dtype))
+    return L.DTYPE[t.dtype]
+
+
+def _rows(t, what):
+    """t as rows of consecutive elements (any pitch); other layouts are copied.  -> (tensor, pitch)."""
+    if t.dim() != 2:
+        raise L.StarGCNError("%s: a matrix of rows expected, got shape %s" % (what, tuple(t.shape)))
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _vector(t, n, dtype, what):
+    if t.dim() != 1 or t.numel() != n or t.dtype != dtype:
+        raise L.StarGCNError("%s: %d values of %s expected, got %s of %s" % (what, n, dtype, tuple(t.shape), t.dtype))
+    return t.contiguous()
+
+
+def _quant_rows(x, weight, residual, norm, eps, what):
+    L.require_current_gpu(x, weight, residual)
+    dt = _dtype_id(x, what)
+    x, ldx = _rows(x, what)
+    rows, dim = x.shape
+    ldr, h = 0, x
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise L.StarGCNError("%s: the residual has to match x (%s of %s), got %s of %s" %
+                                 (what, tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+        residual, ldr = _rows(residual, what)
+        h = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
+    if weight is not None:
+        weight = _vector(weight, dim, weight.dtype if weight.dtype == torch.float32 else x.dtype, what + " weight")
+    codes = torch.empty((rows, dim), dtype=torch.int8, device=x.device)
+    scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    L.check(L.lib().sg_quant_rows_i8_hip(L.ptr(codes), L.ptr(scale), L.ptr(h) if residual is not None else None, L.ptr(x), ldx,
+                                         L.ptr(residual), ldr, L.ptr(weight),
+                                         int(weight is not None and weight.dtype == torch.float32), rows, dim, dt, int(norm),
+                                         float(eps), L.stream_ptr()), what)
+    return codes, scale, h
+
+
+def quantize_rows(x):
+    """x (rows, dim) -> (codes int8, scale (rows) fp32) with x[i] ~ codes[i] * scale[i], scale = max|x[i]| / 127.  What gemm_i8
+    takes: rows of an item table or of a dense layer's weight once, activations a call."""
+    codes, scale, _ = _quant_rows(x, None, None, False, 0.0, "quantize_rows")
+    return codes, scale
+
+
+def rms_norm_i8(x, weight=None, residual=None, eps=1e-6):
+    """h = x (+ residual) in x's type; codes and scale of h / sqrt(mean(h^2) + eps) * weight by rows.  -> (codes int8, scale (rows)
+    fp32, h); without a residual h is x itself.  weight (dim): x's type or fp32.  Inference only: codes have no gradient."""
+    return _quant_rows(x, weight, residual, True, eps, "rms_norm_i8")
+
+
+def gemm_i8(a, a_scale, b, b_scale, bias=None, act=None, slope=0.1, out=None, out_dtype=torch.float32):
+    """out[m, n] = act(a_scale[m] * b_scale[n] * <a[m], b[n]> + bias[n]) on the 8-bit matrix units: a (M, K), b (N, K) codes of
+    quantize_rows / rms_norm_i8 (rows of any pitch), sums exact, out (M, N) fp32, fp16 or bf16."""
+    L.require_current_gpu(a, a_scale, b, b_scale, bias, out)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise L.StarGCNError("gemm_i8: int8 codes expected, got %s and %s" % (a.dtype, b.dtype))
+    a, lda = _rows(a, "gemm_i8 a")
+    b, ldb = _rows(b, "gemm_i8 b")
+    (M, K), (N, Kb) = a.shape, b.shape
+    if K != Kb:
+        raise L.StarGCNError("gemm_i8: inner dimensions differ (%d vs %d)" % (K, Kb))
+    a_scale = _vector(a_scale, M, torch.float32, "gemm_i8 a_scale")
+    b_scale = _vector(b_scale, N, torch.float32, "gemm_i8 b_scale")
+    if bias is not None:
+        bias = _vector(bias, N, torch.float32, "gemm_i8 bias")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or (out.stride(0) < N and M > 1):
+        raise L.StarGCNError("gemm_i8: out has to be (%d, %d) with consecutive elements in a row" % (M, N))
+    dt = _dtype_id(out, "gemm_i8 out")
+    lib = L.lib()
+    wsn = lib.sg_gemm_i8_workspace_bytes(M, N, K)
+    ws = L.scratch(wsn, a.device)
+    L.check(lib.sg_gemm_i8_hip(L.ptr(out), out.stride(0) if M > 1 else max(N, 1), dt, L.ptr(a), lda, L.ptr(a_scale), L.ptr(b), ldb,
+                               L.ptr(b_scale), L.ptr(bias), M, N, K, _act_id(act), float(slope), L.ptr(ws), wsn, L.stream_ptr()),
+            "sg_gemm_i8_hip")
+    return out
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One item a row of logits (rows, items), drawn with the numbers u (rows) in [0, 1): scores over `temperature`, then the
+    top_k best (0: all), of those the best that hold the share top_p of the probability (1: all), of those the ones at least
+    min_p times as likely as the best (0: all).  Each setting is a number, or a tensor with one a row.  -> (ids int32, prob
+    fp32: the drawn item's probability among the kept ones).  Equal scores rank by index; scores of -inf and NaN are never
+    drawn; a row of nothing else gives id -1, prob 0.  The same inputs draw the same items in every run."""
+    L.require_current_gpu(logits, u)
+    dt = _dtype_id(logits, "sample_rows")
+    logits, ld = _rows(logits, "sample_rows")
+    rows, n = logits.shape
+    u = _vector(u, rows, torch.float32, "sample_rows u")
+
+    def setting(v, dtype, name):
+        if not torch.is_tensor(v):
+            return v, None
+        L.require_current_gpu(v)
+        if v.dtype != dtype and v.is_floating_point() != dtype.is_floating_point:
+            raise L.StarGCNError("sample_rows: %s cannot be of %s" % (name, v.dtype))
+        v = v if v.dtype == dtype else v.to(dtype)
+        return 0, _vector(v.view(1) if v.dim() == 0 and rows == 1 else v, rows, dtype, "sample_rows " + name)
+
+    (t, tr), (p, pr), (m, mr) = (setting(v, torch.float32, name) for v, name in
+                                 ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
+    k, kr = setting(top_k, torch.int32, "top_k")
+    ids = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    prob = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    lib = L.lib()
+    wsn = lib.sg_sample_rows_workspace_bytes(rows, n)
+    ws = L.scratch(wsn, logits.device)
+    L.check(lib.sg_sample_rows_hip(L.ptr(ids), L.ptr(prob), L.ptr(logits), ld, dt, L.ptr(u), rows, n, float(t), int(k), float(p),
+                                   float(m), L.ptr(tr), L.ptr(kr), L.ptr(pr), L.ptr(mr), L.ptr(ws), wsn, L.stream_ptr()),
+            "sg_sample_rows_hip")
+    return ids, prob
+
+
+def _distill_shapes(student, teacher, ids):
+    L.require_current_gpu(student, teacher, ids)
+    _dtype_id(student, "distill_loss")
+    if teacher.dim() != 2 or teacher.shape != ids.shape or student.dim() != 2 or teacher.shape[0] != student.shape[0]:
+        raise L.StarGCNError("distill_loss: student (rows, items), teacher scores and ids (rows, k) expected, got %s, %s and %s" %
+                             (tuple(student.shape), tuple(teacher.shape), tuple(ids.shape)))
+
+
+def distill_fwd(student, teacher, ids, scale, temperature=1.0):
+    """-> (loss, stats, p) of sg_distill_hip; functional.distill_loss is the differentiable form."""
+    _distill_shapes(student, teacher, ids)
+    student, ld = _rows(student, "distill_loss")
+    teacher, ids = L.f32c(teacher), L.i32c(ids)
+    (rows, n), k = student.shape, teacher.shape[1]
+    loss = torch.empty((), dtype=torch.float32, device=student.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=student.device)
+    p = torch.empty((rows, k), dtype=torch.float32, device=student.device)
+    lib = L.lib()
+    wsn = lib.sg_distill_workspace_bytes(rows, n)
+    ws = L.scratch(wsn, student.device)
+    L.check(lib.sg_distill_hip(L.ptr(loss), L.ptr(stats), L.ptr(p), L.ptr(student), ld, L.DTYPE[student.dtype], L.ptr(teacher),
+                               L.ptr(ids), rows, n, k, float(temperature), float(scale), L.ptr(ws), wsn, L.stream_ptr()),
+            "sg_distill_hip")
+    return loss, stats, p
+
+
+def distill_bwd(grad_loss, student, stats, p, ids, scale, temperature=1.0):
+    """The gradient of distill_fwd's loss for the student's scores (contiguous, the student's type)."""
+    L.require_current_gpu(grad_loss, student, stats, p, ids)
+    student, ld = _rows(student, "distill_loss")
+    ids = L.i32c(ids)
+    rows, n = student.shape
+    grad = torch.empty((rows, n), dtype=student.dtype, device=student.device)
+    L.check(L.lib().sg_distill_bwd_hip(L.ptr(grad), L.ptr(student), ld, L.DTYPE[student.dtype], L.ptr(stats), L.ptr(p), L.ptr(ids),
+                                       rows, n, p.shape[1], float(temperature), float(scale), L.ptr(L.f32c(grad_loss)),
+                                       L.stream_ptr()), "sg_distill_bwd_hip")
+    return grad

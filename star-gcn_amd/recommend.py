@@ -1,0 +1,45 @@
+"""Answers out of the whole item catalogue: scores of a user's row against every item's row in 8 bits, and items drawn from
+them.  The reference scores given (user, item) pairs only (experiments/STAR-GCN.py:428-438).
+
+    net.eval()
+    with torch.no_grad():
+        users, items = net.rating_rows(plan)
+    head = CatalogueHead(items)                               # once per refresh of the item rows
+    ids, prob = head.draw(users[batch], torch.rand(len(batch), device=users.device), temperature=0.7, top_k=100, seen=seen)
+"""
+import torch
+
+from . import _lib as L
+from . import ops
+
+
+class CatalogueHead(object):
+    """The item rows as 8-bit codes with one scale an item (a quarter of the fp32 rows' bytes).  A score is the inner product of
+    the dequantised rows, summed exactly: |score - <user, item>| <= sum of |u_k| s_i / 2 + |i_k| s_u / 2 + s_u s_i / 4 over k, s = max|row| / 127.
+
+    bias (items) fp32 is added to every score.  With norm_weight (width), user rows pass through the root-mean-square norm
+    first, optionally with a residual: the scores' scale, and so what `temperature` means, is then the same for every user."""
+
+    def __init__(self, item_rows, bias=None, norm_weight=None, eps=1e-6):
+        self.codes, self.scale = ops.quantize_rows(item_rows.detach())
+        self.bias, self.norm_weight, self.eps = bias, norm_weight, eps
+        self.items = self.codes.shape[0]
+
+    def scores(self, user_rows, residual=None, out_dtype=torch.float32):
+        """(users, items) scores."""
+        user_rows = user_rows.detach()
+        if self.norm_weight is not None:
+            codes, scale, _ = ops.rms_norm_i8(user_rows, self.norm_weight, residual=residual, eps=self.eps)
+        elif residual is not None:
+            raise L.StarGCNError("CatalogueHead: a residual needs norm_weight")
+        else:
+            codes, scale = ops.quantize_rows(user_rows)
+        return ops.gemm_i8(codes, scale, self.codes, self.scale, bias=self.bias, out_dtype=out_dtype)
+
+    def draw(self, user_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, residual=None, seen=None):
+        """One item a user row -> (ids int32, prob fp32), see ops.sample_rows.  seen: (rows, items) index pair of what is not to
+        be drawn, e.g. the items that a user has rated; a user who has seen everything gets id -1."""
+        s = self.scores(user_rows, residual=residual)
+        if seen is not None:
+            s[seen[0].long(), seen[1].long()] = -float("inf")
+        return ops.sample_rows(s, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
