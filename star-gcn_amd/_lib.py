@@ -223,10 +223,15 @@ def require_gpu(*tensors):
 
 def require_current_gpu(*tensors):
     """require_gpu, and that every tensor lives on the current device: kernels go to that device's current stream."""
-    require_gpu(*tensors)
-    cur = torch.cuda.current_device()
+    cur = -1
     for t in tensors:
-        if t is not None and t.device.index != cur:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            require_gpu(t)
+        if cur < 0:
+            cur = torch.cuda.current_device()
+        if t.get_device() != cur:
             raise StarGCNError("a tensor is on %s but the current device is cuda:%d (torch.cuda.device selects it)" % (t.device, cur))
 
 
@@ -241,7 +246,7 @@ def ptr(t):
 
 
 def stream_ptr():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 _ws_cache = collections.OrderedDict()

@@ -7,12 +7,18 @@
 // once for each of its two products, once for the bias and once to C's type.
 //
 // Tile kernel.  v_mfma_i32_32x32x32_i8: a lane feeds 16 consecutive k of one row of A and one of B, so both operands are used
-// exactly as they lie in memory.  A K step is 64 bytes of each of the tile's rows.  In LDS a row's four 16-byte chunks sit at
-// slot = chunk ^ ((row >> 1) & 3): the eight rows that a b128 read touches at once then fall on eight different 16-byte bank
-// groups.
-//   * Aligned operands (base and pitch multiples of 16): LDS-DMA, NST stages, one barrier a K step, NST - 1 steps in flight.
-//   * Otherwise, and for the last K step where K % 64 != 0: through registers, out-of-range k as zeros.
+// exactly as they lie in memory.  A K step is 64 or 128 bytes of each of the tile's rows.  In LDS a row's 16-byte chunks sit at
+// slot = chunk ^ swizzle(row), chosen so that the 16 rows that a b128 read touches at once fall on 16 different 16-byte groups
+// of the 64 banks (SQ_LDS_BANK_CONFLICT 0 in the steps; the first choice, for eight rows at once, cost half of the LDS cycles).
+//   * Aligned operands (base and pitch multiples of 16): LDS-DMA by buffer loads, whose addresses are one register a piece and
+//     a scalar step; one barrier a step, the next step's pieces are issued between the last matrix instructions of a step.
+//   * Otherwise, and for the last step where K is no multiple of it: through registers, out-of-range k as zeros.
 // Rows past M or N are read as the last row; nothing is stored for them.
+//
+// What bounds it, measured on an MI355X.  8192 x 8192 x 4096, bf16 out: 281 us, 1.95 POP/s; the same with zero operands 181 us,
+// so it is the chip's power that sets the clock (1.7 GHz in the counters' runs), not the schedule; the matrix units are busy 55 %
+// of the cycles.  A K-short product (10000 x 10677 x 256 into fp32) is bound by its stores: 110 us, 3.9 TB/s against 6.6 TB/s of
+// a fill of the same buffer; odd row lengths cost it 10 %.  One row against 10677: the call's own latency.
 #include "rows_shared.hpp"
 
 #include <algorithm>
@@ -29,7 +35,14 @@ using f16x3::act_fn;
 using f16x3::glb_void;
 using f16x3::lds_void;
 
-constexpr int BK = 64;      // bytes of a row in a K step
+constexpr int GROUP = 8;                   // columns of tiles in a band; 4, 16 and whole rows of tiles were 1 to 2 % slower
+
+// slot of 16-byte chunk c of a row in LDS: c ^ swizzle(row)
+template <int BK>
+__device__ __forceinline__ int swizzle(int row) {
+  static_assert(BK == 64 || BK == 128, "rows of 64 or 128 bytes");
+  return BK == 64 ? (row >> 2) & 3 : (row >> 1) & 7;
+}
 
 struct Args {
   void* C;
@@ -40,8 +53,9 @@ struct Args {
   const float* bias;
   int* ws;                 // split K: [splits][M][N] sums
   long long lda, ldb, ldc;
-  int M, N, K, act, splits, steps_per_split, tiles_m, tiles_n;
+  int M, N, K, act, splits, k_per_split, tiles_m, tiles_n;
   float slope;
+  int nt;                  // store past the caches: C's rows are 16-byte aligned, and C is larger than the Infinity Cache
 };
 
 template <typename T>
@@ -53,7 +67,7 @@ __device__ __forceinline__ void finish(const Args& g, T* c, int sum, float sa, f
 __device__ __forceinline__ i32x4 load_codes(const int8_t* row, int k, int K) {
   i32x4 v = {0, 0, 0, 0};
   if (k + 16 <= K) {
-    __builtin_memcpy(&v, row + k, 16);
+    v = *reinterpret_cast<const vec16_any*>(row + k);
   } else if (k < K) {
     int8_t b[16];
 #pragma unroll
@@ -70,38 +84,58 @@ __device__ __forceinline__ void wait_dma() {
   asm volatile("" ::: "memory");
 }
 
-// tile TM x TN, waves of WM x WN; NST LDS stages; DMA: operands are 16-byte aligned
-template <typename T, int TM, int TN, int WM, int WN, int NST, bool DMA>
+// tile TM x TN, waves of WM x WN, K steps of BK bytes, NST LDS stages; DMA: operands are 16-byte aligned
+template <typename T, int TM, int TN, int WM, int WN, int BK, int NST, bool DMA, bool ACT>
 __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const Args g) {
-  constexpr int NWN = TN / WN, NW = TM / WM * NWN, IM = WM / 32, IN = WN / 32;
-  constexpr int ROWS = TM + TN, STAGE = ROWS * BK, PIECES = ROWS / 16 / NW;      // a piece: 16 rows x 64 bytes, one wave access
-  static_assert(ROWS % (16 * NW) == 0, "pieces divide over the waves");
-  __shared__ __attribute__((aligned(16))) char smem[NST * STAGE];
+  constexpr int NWN = TN / WN, NW = TM / WM * NWN, IM = WM / 32, IN = WN / 32, H = BK / 32;
+  constexpr int CPR = BK / 16, RP = 64 / CPR;                           // 16-byte chunks a row; a piece: RP rows x BK bytes, one wave access
+  constexpr int PA = TM / RP / NW, PB = TN / RP / NW, PIECES = PA + PB, STAGE = (TM + TN) * BK;
+  constexpr int V = 16 / sizeof(T), LPR = WN / V, RPP = 64 / LPR;       // epilogue: lanes a row, rows a pass
+  constexpr int CP = WN + 4, CST = 32 * CP;                             // a wave's part of LDS: 32 rows, padded
+  static_assert(TM % (RP * NW) == 0 && TN % (RP * NW) == 0, "pieces divide over the waves");
+  constexpr int SMEM = NST * STAGE > NW * CST * 4 ? NST * STAGE : NW * CST * 4;
+  __shared__ __attribute__((aligned(16))) char smem[SMEM];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = wave / NWN, wn = wave % NWN;
-  // workgroup b runs on XCD b % 8: give each XCD consecutive tiles, so that those that share rows of A share an L2
+  // workgroup b runs on XCD b % 8: give each XCD consecutive tiles, so that those that share rows share an L2
   const int nt = g.tiles_m * g.tiles_n, z = blockIdx.x / nt, lin = blockIdx.x - z * nt;
   const int q8 = nt >> 3, r8 = nt & 7, x8 = lin & 7;
   const int tile = (x8 < r8 ? x8 * (q8 + 1) : r8 * (q8 + 1) + (x8 - r8) * q8) + (lin >> 3);
-  const int m0 = tile / g.tiles_n * TM, n0 = tile % g.tiles_n * TN;
-  const int s0 = z * g.steps_per_split, s1 = min((g.K + BK - 1) / BK, s0 + g.steps_per_split);
-  const int full = DMA ? min(s1, g.K / BK) : s0;       // steps [s0, full) by DMA, [full, s1) through registers
+  // tiles in bands of GROUP columns, by rows inside a band: the tiles of an XCD at one time share rows of A and of B
+  const int band = tile / (GROUP * g.tiles_m), in_band = tile - band * GROUP * g.tiles_m, width = min(GROUP, g.tiles_n - band * GROUP);
+  const int m0 = in_band / width * TM, n0 = (band * GROUP + in_band % width) * TN;
+  const int k0 = z * g.k_per_split, k1 = min(g.K, k0 + g.k_per_split);  // this split's k; k0 is a multiple of every BK
+  const int steps = (k1 - k0 + BK - 1) / BK, full = DMA ? (k1 - k0) / BK : 0;      // steps [0, full) by DMA, [full, steps) through registers
 
-  // this wave's pieces: lane l moves chunk (l & 3) ^ ((row >> 1) & 3) of row l >> 2 to the piece's byte 16 l
-  const int prow = lane >> 2, pchunk = (lane & 3) ^ ((prow >> 1) & 3);
-  const int8_t* src[PIECES];
+  // this wave's pieces: lane l moves chunk (l % CPR) ^ swizzle(row) of row l / CPR to the piece's byte 16 l
+  const int prow = lane / CPR;
+  const int8_t* pa = g.A + m0 * g.lda + k0;
+  const int8_t* pb = g.B + n0 * g.ldb + k0;
+  const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(pa), 0, 0xffffffffu, 0x00027000);
+  const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(pb), 0, 0xffffffffu, 0x00027000);
+  typename std::conditional<DMA, unsigned, long long>::type off[PIECES];      // by DMA the pitch is bounded
+  auto chunk = [&](int i) { return ((lane % CPR) ^ swizzle<BK>((i < PA ? wave * PA + i : wave * PB + i - PA) * RP + prow)) * 16; };
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int r = (wave * PIECES + i) * 16 + prow;
-    src[i] = r < TM ? g.A + static_cast<long long>(min(m0 + r, g.M - 1)) * g.lda
-                    : g.B + static_cast<long long>(min(n0 + r - TM, g.N - 1)) * g.ldb;
+    const int r = (i < PA ? wave * PA + i : wave * PB + i - PA) * RP + prow;
+    off[i] = (i < PA ? min(r, g.M - 1 - m0) * g.lda : min(r, g.N - 1 - n0) * g.ldb) + (DMA ? chunk(i) : 0);
   }
-  auto issue = [&](int s) {
-    char* st = smem + (s % NST) * STAGE + wave * PIECES * 1024;
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-      __builtin_amdgcn_global_load_lds((glb_void*)(src[i] + s * BK + pchunk * 16), (lds_void*)(st + i * 1024), 16, 0, 0);
+  auto piece = [&](int s, int i) { return smem + (s % NST) * STAGE + (i < PA ? wave * PA + i : TM / RP + wave * PB + i - PA) * 1024; };
+  auto issue = [&](int s, int i) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(i < PA ? ra : rb, (lds_void*)piece(s, i), 16, static_cast<int>(off[i]), s * BK, 0, 0);
   };
+
+  // what the epilogue scales with, loaded ahead of the steps
+  const bool whole = g.splits == 1;
+  const int col = lane % LPR * V, n = n0 + wn * WN + col, room = g.N - n, mw = m0 + wm * WM;
+  float sb[V], bias[V], sa[IM];                        // sa: row lane % 32 of each 32-row block
+#pragma unroll
+  for (int q = 0; q < V; ++q) {
+    sb[q] = whole ? g.sb[min(n + q, g.N - 1)] : 0.f;
+    bias[q] = whole && g.bias ? g.bias[min(n + q, g.N - 1)] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < IM; ++i) sa[i] = whole ? g.sa[min(mw + i * 32 + (lane & 31), g.M - 1)] : 0.f;
 
   i32x16 acc[IM][IN];
 #pragma unroll
@@ -110,70 +144,164 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
     for (int j = 0; j < IN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-  const int l31 = lane & 31, kh = lane >> 5, sw = (l31 >> 1) & 3;      // a fragment row's swizzle: its block starts at a multiple of 32
-  auto multiply = [&](int s) {
-    const char* st = smem + (s % NST) * STAGE;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int slot = ((ks * 2 + kh) ^ sw) * 16;
-      i32x4 a[IM], b[IN];
-#pragma unroll
-      for (int i = 0; i < IM; ++i) a[i] = *reinterpret_cast<const i32x4*>(st + (wm * WM + i * 32 + l31) * BK + slot);
-#pragma unroll
-      for (int j = 0; j < IN; ++j) b[j] = *reinterpret_cast<const i32x4*>(st + (TM + wn * WN + j * 32 + l31) * BK + slot);
-#pragma unroll
-      for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
-    }
+  const int l31 = lane & 31, kh = lane >> 5, sw = swizzle<BK>(l31);     // a fragment's rows start at a multiple of 32
+  const int a_row = (wm * WM + l31) * BK, b_row = (TM + wn * WN + l31) * BK;
+  i32x4 a[2][IM], b[2][IN];                            // fragments of 32 k: one set multiplied, one being read
+  auto read_one = [&](int s, int ks, int f) {
+    const char* st = smem + (s % NST) * STAGE + ((ks * 2 + kh) ^ sw) * 16;
+    if (f < IM) a[ks & 1][f] = *reinterpret_cast<const i32x4*>(st + a_row + f * 32 * BK);
+    else b[ks & 1][f - IM] = *reinterpret_cast<const i32x4*>(st + b_row + (f - IM) * 32 * BK);
   };
-
-  if constexpr (DMA) {
+  auto read = [&](int s, int ks) {
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-      if (s0 + i < full) issue(s0 + i);
-    for (int s = s0; s < full; ++s) {
-      if (s + NST - 2 < full) wait_dma<PIECES * (NST - 2)>();      // the pieces of step s have landed
-      else wait_dma<0>();
-      __builtin_amdgcn_s_barrier();                                // ... for every wave, and step s - 1 has been multiplied
-      asm volatile("" ::: "memory");
-      if (s + NST - 1 < full) issue(s + NST - 1);
-      multiply(s);
-    }
-  }
-  if (full < s1) {
-    i32x4 v[PIECES];
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) v[i] = load_codes(src[i], full * BK + pchunk * 16, g.K);
-    for (int s = full; s < s1; ++s) {
-      __syncthreads();                                             // the stage's last readers are done
-      char* st = smem + (s % NST) * STAGE + wave * PIECES * 1024 + lane * 16;
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) *reinterpret_cast<i32x4*>(st + i * 1024) = v[i];
-      if (s + 1 < s1) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) v[i] = load_codes(src[i], (s + 1) * BK + pchunk * 16, g.K);
-      }
-      __syncthreads();
-      multiply(s);
-    }
-  }
-
-  // epilogue: a lane holds column l31 and rows (e & 3) + 8 (e >> 2) + 4 kh of each 32 x 32 block
-#pragma unroll
-  for (int j = 0; j < IN; ++j) {
-    const int n = n0 + wn * WN + j * 32 + l31;
-    if (n >= g.N) continue;
-    const float sb = g.splits == 1 ? g.sb[n] : 0.f, bias = g.splits == 1 && g.bias ? g.bias[n] : 0.f;
+    for (int f = 0; f < IM + IN; ++f) read_one(s, ks, f);
+  };
+  // between(q) goes before matrix instruction q and stays there: left alone, the compiler moves the reads of the next fragments
+  // down to their use and the matrix units wait for them
+  auto multiply = [&](int ks, auto between) {
 #pragma unroll
     for (int i = 0; i < IM; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int m = m0 + wm * WM + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * kh;
-        if (m >= g.M) continue;
-        if (g.splits == 1) finish(g, static_cast<T*>(g.C) + m * g.ldc + n, acc[i][j][e], g.sa[m], sb, bias);
-        else g.ws[(static_cast<long long>(z) * g.M + m) * g.N + n] = acc[i][j][e];
+      for (int j = 0; j < IN; ++j) {
+        between(i * IN + j);
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks & 1][i], b[ks & 1][j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
+  };
+  auto read_next = [&](int q, int s, int ks) {         // a fragment's share of the reads, in the first half of the matrix instructions
+#pragma unroll
+    for (int f = 0; f < IM + IN; ++f)
+      if (f * IM * IN / (2 * (IM + IN)) == q) read_one(s, ks, f);
+  };
+  auto nothing = [](int) {};
+
+  if constexpr (DMA) {
+    // While 32 k are multiplied the next 32 are read.  The barrier before the last 32 k of step s says that step s + 1 has landed
+    // for every wave and that step s has been read out, whose stage then receives step s + NST.
+    if (full > 0) {
+#pragma unroll
+      for (int p = 0; p < NST; ++p)
+        if (p < full)
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) issue(p, i);
+      if (NST - 1 < full) wait_dma<PIECES * (NST - 1)>();
+      else wait_dma<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      read(0, 0);
+    }
+    auto step = [&](int s, auto more) {                // more: step s + NST exists
+#pragma unroll
+      for (int ks = 0; ks < H - 1; ++ks) {
+        multiply(ks, [&](int q) { read_next(q, s, ks + 1); });
+      }
+      if (more.value || s + 1 < full) {
+        if (more.value || s + NST - 1 < full) wait_dma<PIECES * (NST - 2)>();
+        else wait_dma<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      multiply(H - 1, [&](int q) {
+        if (more.value || s + 1 < full) read_next(q, s + 1, 0);
+        if constexpr (more.value) {
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i)
+            if (i * IM * IN / PIECES == q) issue(s + NST, i);
+        }
+      });
+    };
+    int s = 0;
+    for (; s + NST < full; ++s) step(s, std::true_type{});
+    for (; s < full; ++s) step(s, std::false_type{});
+  }
+  if (full < steps) {
+    i32x4 v[PIECES];
+    auto load = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        v[i] = load_codes((i < PA ? pa : pb) + (off[i] - (DMA ? chunk(i) : 0)), s * BK + chunk(i), k1 - k0);
+    };
+    load(full);
+    for (int s = full; s < steps; ++s) {
+      __syncthreads();                                             // the stage's last readers are done
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) *reinterpret_cast<i32x4*>(piece(s, i) + lane * 16) = v[i];
+      if (s + 1 < steps) load(s + 1);
+      __syncthreads();
+#pragma unroll
+      for (int ks = 0; ks < H; ++ks) {
+        read(s, ks);
+        multiply(ks, nothing);
+      }
+    }
+  }
+
+  // epilogue: 32 rows at a time through the wave's own part of LDS, where a lane's column of sums (column l31, rows
+  // (e & 3) + 8 (e >> 2) + 4 kh of each 32 x 32 block) becomes 16 bytes of a row of C
+  __syncthreads();
+  int* cst = reinterpret_cast<int*>(smem) + wave * CST;
+  const int first = lane / LPR, rows = g.M - mw - first;
+  const auto block = [&](int i, auto use) {            // use(r, sums): row r of the 32, V sums from column `col` on
+#pragma unroll
+    for (int j = 0; j < IN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) cst[((e & 3) + 8 * (e >> 2) + 4 * kh) * CP + j * 32 + l31] = acc[i][j][e];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int UN = ACT ? 1 : 32 / RPP;             // unrolled, the activations' code overflows the instruction cache
+#pragma unroll UN
+    for (int it = 0; it < 32 / RPP; ++it) {
+      int v[V];
+#pragma unroll
+      for (int q = 0; q < V; q += 4) {
+        const i32x4 t4 = *reinterpret_cast<const i32x4*>(cst + (it * RPP + first) * CP + col + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q + e] = t4[e];
+      }
+      use(it * RPP + first, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  const auto finish_all = [&](auto store) {
+    T* o = static_cast<T*>(g.C) + (mw + first) * g.ldc + n;
+    const long long stride = RPP * g.ldc;
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+      block(i, [&](int r, const int* v) {
+        const float sa_r = __shfl(sa[i], r);
+        float f[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          f[q] = fmaf(static_cast<float>(v[q]) * sa_r, sb[q], bias[q]);
+          if (ACT) f[q] = act_fn(f[q], g.act, g.slope);
+        }
+        store(o, f, i * 32 + r - first);
+        o += stride;
+      });
+  };
+  if (!whole) {
+    int* w = g.ws + (static_cast<long long>(z) * g.M + mw + first) * g.N + n;
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+      block(i, [&](int r, const int* v) {
+        if (i * 32 + r - first < rows) {
+#pragma unroll
+          for (int q = 0; q < V; ++q)
+            if (q < room) w[q] = v[q];
+        }
+        w += RPP * g.N;
+      });
+  } else if (m0 + TM <= g.M && n0 + TN <= g.N) {       // nothing to check
+    if (g.nt) finish_all([](T* o, const float* f, int) { store_vec_nt<T, V>(o, f); });
+    else finish_all([](T* o, const float* f, int) { store_vec<T, V>(o, f, V); });
+  } else {
+    finish_all([&](T* o, const float* f, int r) {
+      if (r < rows && room > 0) store_vec<T, V>(o, f, room);
+    });
   }
 }
 
@@ -190,32 +318,49 @@ __global__ __launch_bounds__(256) void gemm_i8_join_kernel(const Args g) {
 }
 
 struct Shape {
-  int tm, tn, splits, steps_per_split;
+  int tm, tn, splits, k_per_split;
 };
 
-// tile and split of K.  Small products are spread over the chip by splitting K while fewer than 256 tiles are at hand and a
-// split keeps at least four steps.
+// The largest tile of which there are enough for all 256 compute units: it moves the fewest operand bytes a product.  Measured
+// (us, tiles of 256 x 256 / 128 x 256 / 128 x 128): 8192 x 8192 x 2048 162 / 185 / 175, 8192 x 8192 x 512 60 / 70 / 69; for K
+// below 512 the epilogue is all, and more and smaller workgroups hide it: 8192 x 8192 x 256 59 / 52 / 54.  Where not even 128 x
+// 128 gives 256 tiles, 32 x 128 (200 x 4096 x 4096: 16 against 27), and K is split while a split keeps 256 k.
 inline Shape shape_of(int64_t M, int64_t N, int64_t K) {
+  auto tiles = [&](int tm, int tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
   Shape s;
-  s.tm = M <= 32 ? 32 : 128;
-  s.tn = 128;
-  const int64_t tiles = (M + s.tm - 1) / s.tm * ((N + s.tn - 1) / s.tn), steps = std::max<int64_t>(1, (K + BK - 1) / BK);
-  int64_t splits = tiles >= 256 ? 1 : std::min<int64_t>(256 / tiles, steps / 4);
-  splits = std::max<int64_t>(1, splits);
-  s.steps_per_split = static_cast<int>((steps + splits - 1) / splits);
-  s.splits = static_cast<int>((steps + s.steps_per_split - 1) / s.steps_per_split);
+  if (K >= 512 && tiles(256, 256) >= 256) s.tm = 256, s.tn = 256;
+  else if (tiles(128, 256) >= 256) s.tm = 128, s.tn = 256;
+  else if (tiles(128, 128) >= 256) s.tm = 128, s.tn = 128;
+  else s.tm = 32, s.tn = 128;
+  const int64_t n = tiles(s.tm, s.tn), steps = std::max<int64_t>(1, (K + 127) / 128);
+  const int64_t splits = n >= 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(256 / n, steps / 2));
+  s.k_per_split = static_cast<int>((steps + splits - 1) / splits * 128);
+  s.splits = static_cast<int>(std::max<int64_t>(1, (K + s.k_per_split - 1) / s.k_per_split));
   return s;
+}
+
+template <typename T, int TM, int TN, int WM, int WN, int BK, int NST, bool DMA>
+void go(const Args& g, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(g.tiles_m * g.tiles_n * g.splits)), block(TM / WM * (TN / WN) * 64);
+  if (g.act == SG_ACT_NONE) hipLaunchKernelGGL((gemm_i8_kernel<T, TM, TN, WM, WN, BK, NST, DMA, false>), grid, block, 0, st, g);
+  else hipLaunchKernelGGL((gemm_i8_kernel<T, TM, TN, WM, WN, BK, NST, DMA, true>), grid, block, 0, st, g);
 }
 
 template <typename T>
 void launch(const Args& g, const Shape& s, bool dma, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(g.tiles_m * g.tiles_n * g.splits));
-  if (s.tm == 32) {
-    if (dma) hipLaunchKernelGGL((gemm_i8_kernel<T, 32, 128, 32, 64, 4, true>), grid, dim3(128), 0, st, g);
-    else hipLaunchKernelGGL((gemm_i8_kernel<T, 32, 128, 32, 64, 2, false>), grid, dim3(128), 0, st, g);
+  if (s.tm == 256) {
+    if (dma) go<T, 256, 256, 128, 64, 128, 2, true>(g, st);
+    else go<T, 256, 256, 128, 64, 64, 2, false>(g, st);
+  } else if (s.tm == 128 && s.tn == 256) {
+    if (dma && g.K >= 512) go<T, 128, 256, 64, 64, 128, 2, true>(g, st);
+    else if (dma) go<T, 128, 256, 64, 64, 64, 2, true>(g, st);
+    else go<T, 128, 256, 64, 64, 64, 2, false>(g, st);
+  } else if (s.tm == 128) {
+    if (dma) go<T, 128, 128, 64, 64, 128, 2, true>(g, st);
+    else go<T, 128, 128, 64, 64, 64, 2, false>(g, st);
   } else {
-    if (dma) hipLaunchKernelGGL((gemm_i8_kernel<T, 128, 128, 64, 64, 3, true>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((gemm_i8_kernel<T, 128, 128, 64, 64, 2, false>), grid, dim3(256), 0, st, g);
+    if (dma) go<T, 32, 128, 32, 64, 64, 4, true>(g, st);
+    else go<T, 32, 128, 32, 64, 64, 2, false>(g, st);
   }
   if (g.splits > 1) {
     const int64_t blocks = std::min<int64_t>(2048, (static_cast<int64_t>(g.M) * g.N + 255) / 256);
@@ -247,12 +392,15 @@ SG_API int sg_gemm_i8_hip(void* C, int64_t ldc, int dtype, const int8_t* A, int6
   if (lda < K || ldb < K || ldc < N) return fail(SG_ERR_INVALID, "gemm_i8: rows overlap");
   const i8::Shape s = i8::shape_of(M, N, K);
   i8::Args g{C, A, B, sa, sb, bias, static_cast<int*>(workspace), lda, ldb, ldc, static_cast<int>(M), static_cast<int>(N),
-             static_cast<int>(K), act, s.splits, s.steps_per_split, static_cast<int>((M + s.tm - 1) / s.tm),
-             static_cast<int>((N + s.tn - 1) / s.tn), slope};
+             static_cast<int>(K), act, s.splits, s.k_per_split, static_cast<int>((M + s.tm - 1) / s.tm),
+             static_cast<int>((N + s.tn - 1) / s.tn), slope, 0};
+  const int size = dtype == SG_DTYPE_F32 ? 4 : 2;
+  // measured at 10000 x 10752 into fp32: 93 us past the caches, 99 through them
+  g.nt = aligned(C, 16) && ldc * size % 16 == 0 && M * N * size > (256ll << 20);
   if (static_cast<int64_t>(g.tiles_m) * g.tiles_n * s.splits >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "gemm_i8: too many tiles");
   if (s.splits > 1 && (!workspace || workspace_bytes < sg_gemm_i8_workspace_bytes(M, N, K)))
     return fail(SG_ERR_WORKSPACE, "gemm_i8 workspace too small");
-  const bool dma = aligned(A, 16) && aligned(B, 16) && lda % 16 == 0 && ldb % 16 == 0 && K >= i8::BK;
+  const bool dma = aligned(A, 16) && aligned(B, 16) && lda % 16 == 0 && ldb % 16 == 0 && lda <= SG_GEMM_I8_MAX_K * 64 && ldb <= SG_GEMM_I8_MAX_K * 64;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == SG_DTYPE_F32) i8::launch<float>(g, s, dma, st);
   else if (dtype == SG_DTYPE_F16) i8::launch<f16>(g, s, dma, st);

@@ -19,26 +19,58 @@ __device__ __forceinline__ float to_f32(bf16 v) { return __uint_as_float(static_
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ f16 from_f32<f16>(float v) { return static_cast<f16>(v); }
-template <> __device__ __forceinline__ bf16 from_f32<bf16>(float v) {      // to nearest, ties to even; NaN stays NaN
-  const unsigned u = __float_as_uint(v);
-  const unsigned r = (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-  return bf16{static_cast<uint16_t>(v != v ? 0x7fc0u : r)};
+template <> __device__ __forceinline__ bf16 from_f32<bf16>(float v) {      // v_cvt_pk_bf16_f32: to nearest, ties to even
+  return __builtin_bit_cast(bf16, static_cast<__bf16>(v));
 }
 template <typename T> __device__ __forceinline__ float round_to(float v) { return to_f32(from_f32<T>(v)); }
 
-// V elements as one vector access.  The hardware takes vector accesses at any byte address; rows of odd length start where
-// they start.
+// V elements as one vector access (4, 8 or 16 bytes a time).  The hardware takes vector accesses at any byte address; rows of odd
+// length start where they start.  The vector types keep the compiler from taking the access apart to share its first element's
+// store with the tail's.
 template <typename T, int V>
-struct __attribute__((packed, aligned(sizeof(T)))) vec_any {
+struct alignas(sizeof(T) * V) pack {
   T v[V];
 };
+typedef int vec16 __attribute__((ext_vector_type(4)));
+typedef vec16 vec16_any __attribute__((aligned(1)));
+typedef int vec8 __attribute__((ext_vector_type(2)));
+typedef vec8 vec8_any __attribute__((aligned(1)));
+typedef int vec4_any __attribute__((aligned(1)));
+
+template <typename T, int V>
+__device__ __forceinline__ pack<T, V> load_pack(const T* p) {
+  constexpr int B = sizeof(T) * V;
+  if constexpr (B == 4) {
+    return __builtin_bit_cast(pack<T, V>, *reinterpret_cast<const vec4_any*>(p));
+  } else if constexpr (B == 8) {
+    return __builtin_bit_cast(pack<T, V>, *reinterpret_cast<const vec8_any*>(p));
+  } else {
+    static_assert(B % 16 == 0, "4, 8 or a multiple of 16 bytes");
+    struct alignas(B) { vec16 q[B / 16]; } a;
+#pragma unroll
+    for (int i = 0; i < B / 16; ++i) a.q[i] = reinterpret_cast<const vec16_any*>(p)[i];
+    return __builtin_bit_cast(pack<T, V>, a);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const pack<T, V>& a) {
+  constexpr int B = sizeof(T) * V;
+  if constexpr (B == 4) {
+    *reinterpret_cast<vec4_any*>(p) = __builtin_bit_cast(int, a);
+  } else if constexpr (B == 8) {
+    *reinterpret_cast<vec8_any*>(p) = __builtin_bit_cast(vec8, a);
+  } else {
+    static_assert(B == 16, "4, 8 or 16 bytes");
+    *reinterpret_cast<vec16_any*>(p) = __builtin_bit_cast(vec16, a);
+  }
+}
 
 // n = V: one vector load; 0 < n < V: element loads, zeros behind them; n <= 0: zeros, nothing is read
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(float* out, const T* p, int n) {
   if (n >= V) {
-    vec_any<T, V> a;
-    __builtin_memcpy(&a, p, sizeof(a));
+    const pack<T, V> a = load_pack<T, V>(p);
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = to_f32(a.v[j]);
   } else {
@@ -49,29 +81,38 @@ __device__ __forceinline__ void load_vec(float* out, const T* p, int n) {
 
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float* in, int n) {
-  if (n >= V) {
-    vec_any<T, V> a;
+  pack<T, V> a;
 #pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(in[j]);
-    __builtin_memcpy(p, &a, sizeof(a));
+  for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(in[j]);
+  if (n >= V) {
+    store_pack<T, V>(p, a);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (j < n) p[j] = from_f32<T>(in[j]);
+      if (j < n) p[j] = a.v[j];
   }
+}
+
+// 16 aligned bytes past the caches: for what nothing reads soon
+template <typename T, int V>
+__device__ __forceinline__ void store_vec_nt(T* p, const float* in) {
+  pack<T, V> a;
+#pragma unroll
+  for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(in[j]);
+  __builtin_nontemporal_store(__builtin_bit_cast(vec16, a), reinterpret_cast<vec16*>(p));
 }
 
 template <int V>
 __device__ __forceinline__ void store_codes(int8_t* p, const int* q, int n) {
-  if (n >= V) {
-    vec_any<int8_t, V> a;
+  pack<int8_t, V> a;
 #pragma unroll
-    for (int j = 0; j < V; ++j) a.v[j] = static_cast<int8_t>(q[j]);
-    __builtin_memcpy(p, &a, sizeof(a));
+  for (int j = 0; j < V; ++j) a.v[j] = static_cast<int8_t>(q[j]);
+  if (n >= V) {
+    store_pack<int8_t, V>(p, a);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (j < n) p[j] = static_cast<int8_t>(q[j]);
+      if (j < n) p[j] = a.v[j];
   }
 }
 
