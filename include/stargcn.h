@@ -673,7 +673,7 @@ int sg_gemm_i8_hip(void* C, int64_t ldc, int dtype, const int8_t* A, int64_t lda
  * top_p 0 or min_p > 1 leave the first item.  Scores of -inf and NaN are never drawn; a row of nothing else gets -1 and 0.
  * Settings are scalars, or one a row where the *_rows pointer is not NULL (values below 0 count as 0 there).  u in [0, 1). */
 #define SG_SAMPLE_MAX_ITEMS (1 << 30)
-size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n);
+size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n, int dtype);
 int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld, int dtype, const float* u, int64_t rows, int64_t n,
                        double temperature, int64_t top_k, double top_p, double min_p, const float* temperature_rows,
                        const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, void* workspace,

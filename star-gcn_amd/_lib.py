@@ -153,7 +153,7 @@ _SIGS = {
     "sg_quant_rows_i8_hip": (_INT, [_P] * 4 + [_I64, _P, _I64, _P, _INT, _I64, _I64, _INT, _INT, _F64, _P]),
     "sg_gemm_i8_workspace_bytes": (_SZ, [_I64] * 3),
     "sg_gemm_i8_hip": (_INT, [_P, _I64, _INT, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _INT, _F32, _P, _SZ, _P]),
-    "sg_sample_rows_workspace_bytes": (_SZ, [_I64] * 2),
+    "sg_sample_rows_workspace_bytes": (_SZ, [_I64, _I64, _INT]),
     "sg_sample_rows_hip": (_INT, [_P, _P, _P, _I64, _INT, _P, _I64, _I64, _F64, _I64, _F64, _F64] + [_P] * 5 + [_SZ, _P]),
     "sg_distill_workspace_bytes": (_SZ, [_I64] * 2),
     "sg_distill_hip": (_INT, [_P] * 4 + [_I64, _INT, _P, _P, _I64, _I64, _I64, _F32, _F32, _P, _SZ, _P]),

@@ -5,13 +5,19 @@
 //   and min-p (w_i >= m) leave, and at least the first item.
 //   drawn: the first item, by index, at which the kept weight summed up to it exceeds u times the kept weight
 //
-// Which item is drawn is a decision at the border of two sums over the catalogue, so a weight is a whole number: w * 2^s, s = min(51, 62 - log2 N), from a 64-bit polynomial.  Sums of whole numbers are exact in any order: the
-// result does not depend on how the row is spread over threads, on the order of the atomic additions, or on the run.  Weights
-// below 2^-(s+1) of the largest are 0 and cannot be drawn.
+// Which item is drawn is a decision at the border of two sums over the catalogue, so a weight is a whole number: w * 2^s, s =
+// min(51, 62 - log2 N), from a 64-bit polynomial.  Sums of whole numbers are exact in any order: the result does not depend on
+// how the row is spread over threads and workgroups, on the order of the atomic additions, or on the run.  Weights below
+// 2^-(s+1) of the largest are 0 and cannot be drawn.
 //
-// The order is never formed.  A histogram of (max l - l) / T, count and weight, shows in which bin a limit falls; the limit's
-// own element is then found among that bin's elements, digit by digit of the score's ordered bits, and among equal scores by
-// index.  -inf and NaN are scores of items that are never drawn; a row without any other draws -1.
+// The order is never formed.  A histogram of (max l - l) / T, count and weight, shows in which bin a limit falls.  The limit's
+// own element is found among that bin's elements, by rank where they are few, else by subdividing the range of their place in
+// the order (score and index in 64 bits, all different) until they are.  -inf and NaN are scores of items that are never drawn;
+// a row without any other draws -1.
+//
+// Rows of up to 16384 items: one workgroup a row, the row in its registers.  Longer rows are cut into pieces, five launches:
+// maximum; histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits
+// and draw.  A list that overflows (many equal scores) is replaced by passes over the row.
 #include "rows_shared.hpp"
 
 #include <algorithm>
@@ -20,8 +26,10 @@ namespace sg {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
-constexpr int kBins = 2048;        // of the histogram, and of an 11-bit digit
-constexpr int kChunks = 4096;      // partial weights by index
+constexpr int kBins = 2048;        // of the histogram and of a subdivision: two a thread
+constexpr int kFew = 512;          // candidates that are ranked against each other
+constexpr int kChunks = 4096;      // partial weights by index of a long row
+constexpr int kMaxPieces = 32;
 
 typedef unsigned long long u64;
 
@@ -37,6 +45,15 @@ struct SampleArgs {
   double t0, p0, m0;
   long long ld, k0;
   int rows, n, bits;               // bits: s above
+  // long rows: pieces of `piece` items, chunks of `span`; workspace
+  int pieces, piece, span, chunks, room;
+  float* tops;                     // (rows, pieces)
+  u64* mass;                       // (rows, pieces, kBins)
+  unsigned* count;
+  struct RowState* state;          // (rows)
+  unsigned* listed;                // (rows, pieces): candidates of the piece, which may be more than `room`
+  u64* list;                       // (rows, pieces, room): their places in the order
+  u64* chunk;                      // (rows, chunks): weight of what is surely kept
 };
 
 struct Row {                       // a row's settings, the same on every thread
@@ -61,11 +78,17 @@ __device__ __forceinline__ Row row_settings(const SampleArgs& g, int row) {
   return r;
 }
 
-// scores as whole numbers in the scores' order (both zeros are the same score; NaN is dealt with before)
-__device__ __forceinline__ unsigned ordered(float l) {
+// an item's place in the order, the largest first: its score as a whole number in the scores' order (both zeros are the same
+// score; NaN is dealt with before) above the complement of its index
+__device__ __forceinline__ u64 place(float l, int i) {
   const unsigned b = __float_as_uint(l + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return static_cast<u64>(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | static_cast<unsigned>(~i);
 }
+__device__ __forceinline__ float score_at(u64 place) {
+  const unsigned k = static_cast<unsigned>(place >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ int index_at(u64 place) { return static_cast<int>(~static_cast<unsigned>(place)); }
 
 // d = (max - l) log2(e) / T, >= 0; NaN and -inf: beyond every weight
 __device__ __forceinline__ double below_top(float l, float top, double c) {
@@ -98,21 +121,31 @@ __device__ __forceinline__ u64 whole(double w) {              // w < 2^52
 
 __device__ __forceinline__ int bin_of(double d, double scale) { return static_cast<int>(fmin(d * scale, kBins - 1.0)); }
 
-// where the kept items of one limit end: scores above `key`, and those equal to it up to index `last`
-struct Limit {
-  unsigned key;
-  int last;
+
+// a row's scale: what turns a score into a bin and a weight
+struct Scale {
+  float top;
+  double c, bins;
+  int bits;
+  __device__ __forceinline__ double below(float l) const { return below_top(l, top, c); }
+  __device__ __forceinline__ int bin(double d) const { return bin_of(d, bins); }
+  __device__ __forceinline__ double weight(double d) const { return scaled_weight(d, bits); }
 };
+__device__ __forceinline__ Scale scale_of(float top, const Row& r, int bits) {
+  return Scale{top, r.c, (kBins - 1.0) / (bits + 1.0), bits};      // the last bin holds items of weight 0 only
+}
 
-__device__ __forceinline__ bool inside(const Limit& lim, unsigned key, int i) { return key > lim.key || (key == lim.key && i <= lim.last); }
-
-struct Shared {
+struct Histogram {
   u64 mass[kBins];
   unsigned count[kBins];
-  u64 wave_mass[kWaves];
-  unsigned wave_count[kWaves];
-  u64 before_mass;
-  unsigned before_count;
+};
+
+struct Shared {
+  Histogram sub;                   // of a subdivision
+  u64 few_place[kFew], few_weight[kFew];
+  u64 wave_a[kWaves], wave_b[kWaves];
+  u64 before_mass, limit, limit_mass;
+  unsigned before_count, few;
   int found;
 };
 
@@ -132,17 +165,17 @@ __device__ __forceinline__ u64 wave_before(u64 v) {
   return s - v;
 }
 
-// The bin of sh.count / sh.mass, counted from bin 0 on, in which the sum of counts reaches `need` (by_mass: the sum of weights
-// reaches `need`): its number, or kBins, with the sums of the bins before it.  Two bins a thread.
-__device__ __forceinline__ int find_bin(Shared& sh, bool by_mass, u64 need, unsigned& before_count, u64& before_mass) {
+// The bin, counted from bin 0 on, in which the sum of counts reaches `need` (by_mass: the sum of weights), and the sums before
+// it; kBins if there is none.  Two bins a thread.
+__device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, bool by_mass, u64 need, unsigned& before_count, u64& before_mass) {
   const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
-  if (t == 0) sh.found = kBins;
-  const u64 m0 = sh.mass[2 * t], m1 = sh.mass[2 * t + 1];
-  const unsigned c0 = sh.count[2 * t], c1 = sh.count[2 * t + 1];
+  if (t == 0) sh.found = kBins, sh.before_count = 0, sh.before_mass = 0;
+  const u64 m0 = h.mass[2 * t], m1 = h.mass[2 * t + 1];
+  const unsigned c0 = h.count[2 * t], c1 = h.count[2 * t + 1];
   u64 mb = wave_before(m0 + m1), cb = wave_before(static_cast<u64>(c0) + c1);
-  if (lane == kWave - 1) sh.wave_mass[wave] = mb + m0 + m1, sh.wave_count[wave] = static_cast<unsigned>(cb) + c0 + c1;
+  if (lane == kWave - 1) sh.wave_a[wave] = mb + m0 + m1, sh.wave_b[wave] = cb + c0 + c1;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) mb += sh.wave_mass[i], cb += sh.wave_count[i];
+  for (int i = 0; i < wave; ++i) mb += sh.wave_a[i], cb += sh.wave_b[i];
   const u64 a = by_mass ? mb : cb, v0 = by_mass ? m0 : c0, v1 = by_mass ? m1 : c1;
   if (a < need && need <= a + v0) sh.found = 2 * t, sh.before_count = static_cast<unsigned>(cb), sh.before_mass = mb;
   else if (a + v0 < need && need <= a + v0 + v1) sh.found = 2 * t + 1, sh.before_count = static_cast<unsigned>(cb) + c0, sh.before_mass = mb + m0;
@@ -153,208 +186,536 @@ __device__ __forceinline__ int find_bin(Shared& sh, bool by_mass, u64 need, unsi
   return found;
 }
 
-__device__ __forceinline__ void clear_bins(Shared& sh) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) sh.mass[i] = 0, sh.count[i] = 0;
+__device__ __forceinline__ void clear(Histogram& h) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) h.mass[i] = 0, h.count[i] = 0;
   __syncthreads();
 }
 
-// f(score, index) for every element of the row, any order
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T* row, int n, F f) {
-  constexpr int V = 16 / sizeof(T);
-  for (int base = threadIdx.x * V; base < n; base += kThreads * V) {
-    float x[V];
-    load_vec<T, V>(x, row + base, n - base);
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (base + j < n) f(x[j], base + j);
-  }
+template <typename Src>
+__device__ __forceinline__ void fill(Histogram& h, const Src& src, const Scale& sc, bool masses) {
+  clear(h);
+  src([&](float l, int) {
+    const double d = sc.below(l);
+    if (d == __builtin_inf()) return;
+    const int b = sc.bin(d);
+    atomicAdd(&h.count[b], 1u);
+    const u64 w = masses ? whole(sc.weight(d)) : 0;
+    if (w) atomicAdd(&h.mass[b], w);
+  });
+  __syncthreads();
 }
 
-// The limit inside bin `bin`, of which the order's items before it number `count` and weigh `mass`: by count, the item with
-// which the count reaches `need`; by mass, the last item before which the weight is below `need`.  On return count and mass
-// include the limit's own item.
-template <typename T>
-__device__ __forceinline__ Limit find_limit(Shared& sh, const T* row, const SampleArgs& g, float top, double c, double bin_scale, int bin,
-                                            bool by_mass, u64 need, unsigned& count, u64& mass) {
-  unsigned key = 0, here = 0;
-  u64 weight = 0;
+// total weight of a histogram, on every thread
+__device__ __forceinline__ u64 total_mass(Shared& sh, const Histogram& h) {
+  const u64 v = wave_sum(h.mass[2 * threadIdx.x] + h.mass[2 * threadIdx.x + 1]);
+  if (threadIdx.x % kWave == 0) sh.wave_a[threadIdx.x / kWave] = v;
+  __syncthreads();
+  u64 s = 0;
 #pragma unroll
-  for (int level = 0; level < 3; ++level) {              // digits of 11, 11 and 10 bits, the largest digit first
-    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11;
-    clear_bins(sh);
-    each(row, g.n, [&](float l, int) {
-      const double d = below_top(l, top, c);
-      const unsigned k = ordered(l);
-      if (bin_of(d, bin_scale) != bin || d == __builtin_inf() || (level > 0 && (k >> (shift + width)) != (key >> (shift + width)))) return;
-      const unsigned digit = ((1u << width) - 1) - ((k >> shift) & ((1u << width) - 1));
-      atomicAdd(&sh.count[digit], 1u);
-      atomicAdd(&sh.mass[digit], whole(scaled_weight(d, g.bits)));
+  for (int i = 0; i < kWaves; ++i) s += sh.wave_a[i];
+  __syncthreads();
+  return s;
+}
+
+__device__ __forceinline__ u64 share(double p, u64 total) {        // the weight that top-p asks for
+  const u64 need = static_cast<u64>(ceil(p * static_cast<double>(total)));
+  return min(max(need, u64{1}), total);
+}
+
+// The limit among the n items of `src` in bins lo_bin .. hi_bin, before which `count` items of weight `mass` stand in the order:
+// by count, the item with which the count reaches `need`; by mass, the item with which the weight does.  -> its place; mass:
+// with the item itself.
+template <typename Src>
+__device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, unsigned n, bool by_mass,
+                                          u64 need, unsigned count, u64& mass) {
+  const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  u64 lo = 0, hi = ~u64{0};
+  auto members = [&](auto f) {
+    src([&](float l, int i) {
+      const double d = sc.below(l);
+      if (d == __builtin_inf()) return;
+      const int b = sc.bin(d);
+      if (b < lo_bin || b > hi_bin) return;
+      const u64 at = place(l, i);
+      if (at >= lo && at <= hi) f(at, d);
+    });
+  };
+  if (n > kFew) {                                        // the range they span
+    u64 least = ~u64{0}, most = 0;
+    members([&](u64 at, double) { least = min(least, at), most = max(most, at); });
+    for (int off = 32; off > 0; off >>= 1) {
+      least = min(least, static_cast<u64>(__shfl_xor(least, off)));
+      most = max(most, static_cast<u64>(__shfl_xor(most, off)));
+    }
+    if (lane == 0) sh.wave_a[wave] = least, sh.wave_b[wave] = most;
+    __syncthreads();
+    lo = sh.wave_a[0], hi = sh.wave_b[0];
+    for (int i = 1; i < kWaves; ++i) lo = min(lo, sh.wave_a[i]), hi = max(hi, sh.wave_b[i]);
+  }
+  while (n > kFew) {                                     // all places differ: every turn leaves at most 1 / 2048 of the range
+    const int shift = max(0, 53 - __clzll(static_cast<long long>(hi - lo)));
+    clear(sh.sub);
+    members([&](u64 at, double d) {
+      const int digit = static_cast<int>((hi - at) >> shift);
+      atomicAdd(&sh.sub.count[digit], 1u);
+      const u64 w = whole(sc.weight(d));
+      if (w) atomicAdd(&sh.sub.mass[digit], w);
     });
     __syncthreads();
     unsigned bc;
     u64 bm;
-    const int digit = find_bin(sh, by_mass, need - (by_mass ? mass : count), bc, bm);
-    here = sh.count[digit], weight = sh.mass[digit];
-    __syncthreads();
-    key |= (((1u << width) - 1) - digit) << shift;
+    const int digit = min(find_bin(sh, sh.sub, by_mass, need - (by_mass ? mass : count), bc, bm), kBins - 1);
+    n = sh.sub.count[digit];
     count += bc, mass += bm;
-  }
-  // `here` items share the score: equal weights, taken by index
-  const u64 one = weight / here;
-  const unsigned take = by_mass ? static_cast<unsigned>(one ? (need - mass + one - 1) / one : here) : static_cast<unsigned>(need - count);
-  Limit lim{key, 0x7fffffff};
-  count += take, mass += one * take;
-  if (take >= here) return lim;
-  unsigned left = take, index = 0;
-#pragma unroll
-  for (int level = 0; level < 3; ++level) {
-    const int shift = level == 0 ? 20 : level == 1 ? 9 : 0, width = level == 2 ? 9 : 11;
-    clear_bins(sh);
-    each(row, g.n, [&](float l, int i) {
-      if (l != l || ordered(l) != key || (level > 0 && (static_cast<unsigned>(i) >> (shift + width)) != (index >> (shift + width)))) return;
-      atomicAdd(&sh.count[(static_cast<unsigned>(i) >> shift) & ((1u << width) - 1)], 1u);
-    });
+    hi -= static_cast<u64>(digit) << shift;
+    lo = max(lo, hi - ((u64{1} << shift) - 1));
     __syncthreads();
-    unsigned bc;
-    u64 bm;
-    const int digit = find_bin(sh, false, left, bc, bm);
-    left -= bc;
-    index |= static_cast<unsigned>(digit) << shift;
   }
-  lim.last = static_cast<int>(index);
-  return lim;
+  if (t == 0) sh.few = 0, sh.limit = lo, sh.limit_mass = mass;
+  __syncthreads();
+  members([&](u64 at, double d) {
+    const unsigned k = atomicAdd(&sh.few, 1u);
+    if (k < kFew) sh.few_place[k] = at, sh.few_weight[k] = whole(sc.weight(d));
+  });
+  __syncthreads();
+  // each against all: `team` threads a candidate
+  const int m = min(static_cast<int>(sh.few), kFew);
+  int team = kWave;
+  while (team * m > kThreads) team >>= 1;
+  const int me = t / team;
+  u64 cb = 0, mb = 0;
+  const u64 at = me < m ? sh.few_place[me] : 0;
+  if (me < m)
+    for (int j = t % team; j < m; j += team)
+      if (sh.few_place[j] > at) cb += 1, mb += sh.few_weight[j];
+  for (int off = 1; off < team; off <<= 1) cb += __shfl_xor(cb, off), mb += __shfl_xor(mb, off);
+  if (me < m && t % team == 0) {
+    const u64 w = sh.few_weight[me], before = by_mass ? mass + mb : count + cb, own = by_mass ? w : 1;
+    if (before < need && need <= before + own) sh.limit = at, sh.limit_mass = mass + mb + w;
+  }
+  __syncthreads();
+  mass = sh.limit_mass;
+  const u64 limit = sh.limit;
+  __syncthreads();
+  return limit;
 }
 
-// one workgroup a row
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs g) {
+// the weight of an item if it is kept: its place is not below `limit`, the lower of the limits
+__device__ __forceinline__ u64 kept(float l, int i, const Scale& sc, u64 limit, double min_weight) {
+  const double d = sc.below(l);
+  if (!(d < sc.bits + 1.0) || place(l, i) < limit) return 0;
+  const double w = sc.weight(d);
+  return w >= min_weight ? whole(w) : 0;
+}
+
+__device__ __forceinline__ u64 goal_of(float u, u64 total) {       // drawn: the first item with more than this up to it
+  const double x = u;
+  const u64 goal = x > 0.0 ? static_cast<u64>(fmin(x, 1.0) * static_cast<double>(total)) : 0;
+  return min(goal, total - 1);
+}
+
+// The wave's V items a lane, kept weights w: where the sum from `before` on passes `goal`, that lane writes the item.  -> whether
+// some lane did; before is moved on.
+template <int V>
+__device__ __forceinline__ bool draw(const SampleArgs& g, int row, int base, const u64 (&w)[V], u64 goal, u64 total, u64& before) {
+  u64 sum = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum += w[j];
+  u64 b = before + wave_before(sum);
+  const bool hit = b <= goal && goal < b + sum;
+  if (hit) {
+    bool done = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!done && goal < b + w[j]) {
+        g.ids[row] = base + j;
+        g.prob[row] = static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total));
+        done = true;
+      }
+      b += w[j];
+    }
+  }
+  if (__ballot(hit)) return true;
+  before += wave_sum(sum);
+  return false;
+}
+
+__device__ __forceinline__ float group_max(float v, float* red) {
+  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = red[0];
+  for (int i = 1; i < static_cast<int>(blockDim.x) / kWave; ++i) v = fmaxf(v, red[i]);
+  return v;
+}
+
+// ---- one workgroup a row, NV vectors of scores a thread ---------------------------------------------------------------------
+template <typename T, int NV>
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g) {
   __shared__ Shared sh;
-  __shared__ u64 chunk[kChunks];
+  __shared__ Histogram hist;
   __shared__ float red[kWaves];
   constexpr int V = 16 / sizeof(T);
   const int row = blockIdx.x, t = threadIdx.x, wave = t / kWave, lane = t % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   const Row r = row_settings(g, row);
-
+  float x[NV][V];
   float top = -__builtin_inff();
-  each(l, g.n, [&](float x, int) { top = fmaxf(top, x); });
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-  top = red[0];
-  for (int i = 1; i < kWaves; ++i) top = fmaxf(top, red[i]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int base = (i * kThreads + t) * V, n = g.n - base;
+    load_vec<T, V>(x[i], l + base, n);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (j >= n) x[i][j] = -__builtin_inff();
+      top = fmaxf(top, x[i][j]);
+    }
+  }
+  top = group_max(top, red);
   if (top == -__builtin_inff()) {                        // nothing to draw from (also N = 0)
     if (t == 0) g.ids[row] = -1, g.prob[row] = 0.f;
     return;
   }
-
-  // limits.  The last bin holds items of weight 0 only: a limit there keeps every weight.
-  Limit by_k{0, 0x7fffffff}, by_p{0, 0x7fffffff};
+  const Scale sc = scale_of(top, r, g.bits);
+  auto src = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) f(x[i][j], (i * kThreads + t) * V + j);
+  };
+  u64 limit = 0;
   if (r.k > 0 || r.by_p) {
-    const double bin_scale = (kBins - 1.0) / (g.bits + 1.0);
-    auto histogram = [&]() {
-      clear_bins(sh);
-      each(l, g.n, [&](float x, int) {
-        const double d = below_top(x, top, r.c);
-        if (d == __builtin_inf()) return;
-        const int b = bin_of(d, bin_scale);
-        atomicAdd(&sh.count[b], 1u);
-        const u64 w = whole(scaled_weight(d, g.bits));
-        if (w) atomicAdd(&sh.mass[b], w);
-      });
-      __syncthreads();
-    };
-    histogram();
-    u64 total = 0;
-    for (int i = lane; i < kBins; i += kWave) total += sh.mass[i];
-    total = wave_sum(total);
-    __syncthreads();
-    unsigned count = 0;
-    u64 mass = 0;
+    fill(hist, src, sc, r.by_p);
+    unsigned count;
+    u64 mass, total = r.by_p ? total_mass(sh, hist) : 0;
     if (r.k > 0) {
-      const int b = find_bin(sh, false, static_cast<u64>(r.k), count, mass);
+      const int b = find_bin(sh, hist, false, static_cast<u64>(r.k), count, mass);
       if (b < kBins - 1) {
-        by_k = find_limit(sh, l, g, top, r.c, bin_scale, b, false, static_cast<u64>(r.k), count, mass);
+        limit = find_limit(sh, src, sc, b, b, hist.count[b], false, static_cast<u64>(r.k), count, mass);
         total = mass;
-        if (r.by_p) histogram();
       }
     }
     if (r.by_p) {
-      const u64 need = max(u64{1}, static_cast<u64>(ceil(r.p * static_cast<double>(total))));
-      const int b = find_bin(sh, true, need, count, mass);
-      if (b < kBins - 1) by_p = find_limit(sh, l, g, top, r.c, bin_scale, b, true, need, count, mass);
+      const u64 need = share(r.p, total);
+      const int b = find_bin(sh, hist, true, need, count, mass);
+      if (b < kBins - 1) limit = max(limit, find_limit(sh, src, sc, b, b, hist.count[b], true, need, count, mass));
     }
   }
-
-  // kept weight by index: one wave a chunk of 64 V * 2^j items
-  auto weight = [&](float x, int i) -> u64 {
-    const double d = below_top(x, top, r.c);
-    if (!(d < g.bits + 1.0)) return 0;
-    const unsigned key = ordered(x);
-    if (!inside(by_k, key, i) || !inside(by_p, key, i)) return 0;
-    const double w = scaled_weight(d, g.bits);
-    return w >= r.m ? whole(w) : 0;
-  };
-  int span = kWave * V;
-  while ((g.n + span - 1) / span > kChunks) span *= 2;
-  const int chunks = (g.n + span - 1) / span;
-  for (int ch = wave; ch < chunks; ch += kWaves) {
+  // kept weight by index: level i of wave w comes after level i of wave w - 1, and after every wave's level i - 1
+  __shared__ u64 part[NV * kWaves];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
     u64 sum = 0;
-    const int end = min(g.n, (ch + 1) * span);
-    for (int base = ch * span + lane * V; base < end; base += kWave * V) {
-      float x[V];
-      load_vec<T, V>(x, l + base, end - base);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum += kept(x[i][j], (i * kThreads + t) * V + j, sc, limit, r.m);
+    sum = wave_sum(sum);
+    if (lane == 0) part[i * kWaves + wave] = sum;
+  }
+  __syncthreads();
+  static_assert(NV * kWaves <= kWave, "one lane a part");
+  const u64 mine = lane < NV * kWaves ? part[lane] : 0, total = wave_sum(mine), goal = goal_of(g.u[row], total);
+  u64 before = wave_before(mine);
+  const int owner = __ffsll(static_cast<unsigned long long>(__ballot(before <= goal && goal < before + mine))) - 1;
+  if (owner % kWaves != wave) return;
+  before = __shfl(before, owner);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (owner / kWaves == i) {
+      u64 w[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = kept(x[i][j], (i * kThreads + t) * V + j, sc, limit, r.m);
+      draw<V>(g, row, (i * kThreads + t) * V, w, goal, total, before);
+    }
+}
+
+// ---- long rows ----------------------------------------------------------------------------------------------------------------
+
+struct RowState {
+  u64 total, k_mass, p_mass;       // weight of the row; before the top-k bin; before the top-p bins
+  unsigned k_count, k_items, p_items;      // items before the top-k bin, in it, in the top-p bins
+  int k_bin, p_lo, p_hi;           // kBins: no such limit
+};
+
+// f(score, index) for the items [lo, hi) of a row, `threads` threads
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T* row, int lo, int hi, F f) {
+  constexpr int V = 16 / sizeof(T), U = 2;
+  const int step = blockDim.x * V;
+  for (int base = lo + threadIdx.x * V; base < hi; base += U * step) {
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_vec<T, V>(x[u], row + base + u * step, hi - (base + u * step));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (base + j < end) sum += weight(x[j], base + j);
+        if (base + u * step + j < hi) f(x[u][j], base + u * step + j);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void sample_top_kernel(const SampleArgs g) {
+  __shared__ float red[4];
+  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, lo = z * g.piece;
+  float top = -__builtin_inff();
+  each(static_cast<const T*>(g.l) + row * g.ld, lo, min(g.n, lo + g.piece), [&](float x, int) { top = fmaxf(top, x); });
+  top = group_max(top, red);
+  if (threadIdx.x == 0) g.tops[blockIdx.x] = top;
+}
+
+__device__ __forceinline__ float row_top(const SampleArgs& g, int row) {
+  float top = g.tops[row * g.pieces];
+  for (int i = 1; i < g.pieces; ++i) top = fmaxf(top, g.tops[row * g.pieces + i]);
+  return top;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const SampleArgs g) {
+  __shared__ Histogram hist;
+  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, lo = z * g.piece, hi = min(g.n, lo + g.piece);
+  const Row r = row_settings(g, row);
+  if (!(r.k > 0 || r.by_p)) return;
+  const T* l = static_cast<const T*>(g.l) + row * g.ld;
+  fill(hist, [&](auto f) { each(l, lo, hi, f); }, scale_of(row_top(g, row), r, g.bits), r.by_p || r.k > 0);
+  u64* mass = g.mass + static_cast<long long>(blockIdx.x) * kBins;
+  unsigned* count = g.count + static_cast<long long>(blockIdx.x) * kBins;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = hist.mass[i], count[i] = hist.count[i];
+}
+
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs g) {
+  __shared__ Shared sh;
+  __shared__ Histogram hist;
+  const int row = blockIdx.x, t = threadIdx.x;
+  const Row r = row_settings(g, row);
+  RowState s{0, 0, 0, 0, 0, 0, kBins, kBins, kBins};
+  if (r.k > 0 || r.by_p) {
+    for (int i = t; i < kBins; i += kThreads) {
+      u64 m = 0;
+      unsigned c = 0;
+      for (int z = 0; z < g.pieces; ++z) {
+        const long long at = (static_cast<long long>(row) * g.pieces + z) * kBins + i;
+        m += g.mass[at], c += g.count[at];
+      }
+      hist.mass[i] = m, hist.count[i] = c;
+    }
+    __syncthreads();
+    s.total = total_mass(sh, hist);
+    u64 least = s.total, most = s.total;                 // weight of the top-k items
+    if (r.k > 0) {
+      const int b = find_bin(sh, hist, false, static_cast<u64>(r.k), s.k_count, s.k_mass);
+      if (b < kBins - 1) s.k_bin = b, s.k_items = hist.count[b], least = s.k_mass, most = s.k_mass + hist.mass[b];
+    }
+    if (r.by_p && s.total > 0) {                         // total = 0: a row of nothing but -inf and NaN
+      unsigned c;
+      u64 m;
+      s.p_hi = find_bin(sh, hist, true, share(r.p, most), c, m);
+      s.p_hi = min(s.p_hi, kBins - 1);
+      s.p_lo = least > 0 ? min(find_bin(sh, hist, true, share(r.p, least), c, s.p_mass), s.p_hi) : 0;
+      if (least == 0) s.p_mass = 0;
+      u64 items = 0;
+      for (int i = t; i < kBins; i += kThreads)
+        if (i >= s.p_lo && i <= s.p_hi) items += hist.count[i];
+      items = wave_sum(items);
+      if (t % kWave == 0) sh.wave_a[t / kWave] = items;
+      __syncthreads();
+      for (int i = 0; i < kWaves; ++i) s.p_items += static_cast<unsigned>(sh.wave_a[i]);
+    }
+  }
+  if (t == 0) g.state[row] = s;
+}
+
+__device__ __forceinline__ bool surely_kept(const RowState& s, int bin) { return bin < s.k_bin && bin < s.p_lo; }
+__device__ __forceinline__ bool candidate(const RowState& s, int bin) { return bin == s.k_bin || (bin >= s.p_lo && bin <= s.p_hi); }
+
+// one wave a chunk of the piece
+template <typename T>
+__global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) {
+  __shared__ unsigned listed;
+  constexpr int V = 16 / sizeof(T), U = 4;
+  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const T* l = static_cast<const T*>(g.l) + row * g.ld;
+  const Row r = row_settings(g, row);
+  const Scale sc = scale_of(row_top(g, row), r, g.bits);
+  RowState s{0, 0, 0, 0, 0, 0, kBins, kBins, kBins};
+  if (r.k > 0 || r.by_p) s = g.state[row];
+  u64* list = g.list + static_cast<long long>(blockIdx.x) * g.room;
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  const int c0 = z * (g.piece / g.span), c1 = min(g.chunks, c0 + g.piece / g.span);
+  for (int ch = c0 + wave; ch < c1; ch += 4) {
+    u64 sum = 0;
+    const int end = min(g.n, (ch + 1) * g.span);
+    for (int base = ch * g.span + lane * V; base < end; base += U * kWave * V) {
+      float x[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_vec<T, V>(x[u], l + base + u * kWave * V, end - (base + u * kWave * V));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int i = base + u * kWave * V + j;
+          const double d = i < end ? sc.below(x[u][j]) : __builtin_inf();
+          if (!(d < sc.bits + 1.0)) continue;
+          const int b = sc.bin(d);
+          if (surely_kept(s, b)) {
+            const double w = sc.weight(d);
+            if (w >= r.m) sum += whole(w);
+          } else if (candidate(s, b)) {
+            const unsigned k = atomicAdd(&listed, 1u);
+            if (k < static_cast<unsigned>(g.room)) list[k] = place(x[u][j], i);
+          }
+        }
     }
     sum = wave_sum(sum);
-    if (lane == 0) chunk[ch] = sum;
+    if (lane == 0) g.chunk[static_cast<long long>(row) * g.chunks + ch] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) g.listed[blockIdx.x] = listed;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs g) {
+  __shared__ Shared sh;
+  __shared__ u64 chunk[kChunks];
+  constexpr int V = 16 / sizeof(T);
+  const int row = blockIdx.x, t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  const T* l = static_cast<const T*>(g.l) + row * g.ld;
+  const Row r = row_settings(g, row);
+  const float top = row_top(g, row);
+  if (top == -__builtin_inff()) {
+    if (t == 0) g.ids[row] = -1, g.prob[row] = 0.f;
+    return;
+  }
+  const Scale sc = scale_of(top, r, g.bits);
+  RowState s{0, 0, 0, 0, 0, 0, kBins, kBins, kBins};
+  if (r.k > 0 || r.by_p) s = g.state[row];
+  for (int i = t; i < g.chunks; i += kThreads) chunk[i] = g.chunk[static_cast<long long>(row) * g.chunks + i];
+  u64 limit = 0;
+  if (s.k_bin < kBins || s.p_lo < kBins) {
+    bool whole_list = true;
+    for (int z = 0; z < g.pieces; ++z) whole_list = whole_list && g.listed[row * g.pieces + z] <= static_cast<unsigned>(g.room);
+    auto limits = [&](auto src) {
+      u64 mass = s.k_mass, total = s.total;
+      if (s.k_bin < kBins) {
+        limit = find_limit(sh, src, sc, s.k_bin, s.k_bin, s.k_items, false, static_cast<u64>(r.k), s.k_count, mass);
+        total = mass;
+      }
+      if (s.p_lo < kBins) {
+        mass = s.p_mass;
+        limit = max(limit, find_limit(sh, src, sc, s.p_lo, s.p_hi, s.p_items, true, share(r.p, total), 0, mass));
+      }
+    };
+    if (whole_list) {
+      auto src = [&](auto f) {
+        for (int z = 0; z < g.pieces; ++z) {
+          const u64* list = g.list + (static_cast<long long>(row) * g.pieces + z) * g.room;
+          const int n = static_cast<int>(g.listed[row * g.pieces + z]);
+          for (int i = t; i < n; i += kThreads) {
+            const u64 at = list[i];
+            f(score_at(at), index_at(at));
+          }
+        }
+      };
+      limits(src);
+      __syncthreads();
+      src([&](float x, int i) {
+        const u64 w = kept(x, i, sc, limit, r.m);
+        if (w) atomicAdd(&chunk[i / g.span], w);
+      });
+    } else {                                             // too many candidates for the list: over the row itself
+      limits([&](auto f) { each(l, 0, g.n, f); });
+      __syncthreads();
+      for (int ch = wave; ch < g.chunks; ch += kWaves) {
+        u64 sum = 0;
+        const int end = min(g.n, (ch + 1) * g.span);
+        for (int base = ch * g.span + lane * V; base < end; base += kWave * V) {
+          float x[V];
+          load_vec<T, V>(x, l + base, end - base);
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (base + j < end) sum += kept(x[j], base + j, sc, limit, r.m);
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) chunk[ch] = sum;
+      }
+    }
   }
   __syncthreads();
   if (wave != 0) return;
   // the chunk, then the item, at which the sum passes the drawn share
-  const int per = (chunks + kWave - 1) / kWave, c0 = min(chunks, lane * per), c1 = min(chunks, c0 + per);
+  const int per = (g.chunks + kWave - 1) / kWave, c0 = min(g.chunks, lane * per), c1 = min(g.chunks, c0 + per);
   u64 mine = 0;
   for (int i = c0; i < c1; ++i) mine += chunk[i];
-  const u64 total = wave_sum(mine);
-  const double u = g.u[row];
-  u64 goal = u > 0.0 ? static_cast<u64>(fmin(u, 1.0) * static_cast<double>(total)) : 0;
-  goal = min(goal, total - 1);
+  const u64 total = wave_sum(mine), goal = goal_of(g.u[row], total);
   u64 before = wave_before(mine);
   int at = -1;
-  if (before <= goal && goal < before + mine) {
+  if (before <= goal && goal < before + mine)
     for (at = c0; before + chunk[at] <= goal; ++at) before += chunk[at];
-  }
-  const u64 has = __ballot(at >= 0);
-  const int owner = __ffsll(has) - 1;
+  const int owner = __ffsll(static_cast<unsigned long long>(__ballot(at >= 0))) - 1;
   at = __shfl(at, owner);
   before = __shfl(before, owner);
-  const int end = min(g.n, (at + 1) * span);
-  for (int base0 = at * span; base0 < end; base0 += kWave * V) {
+  const int end = min(g.n, (at + 1) * g.span);
+  for (int base0 = at * g.span; base0 < end; base0 += kWave * V) {
     const int base = base0 + lane * V;
     float x[V];
     load_vec<T, V>(x, l + base, end - base);
-    u64 w[V], sum = 0;
+    u64 w[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = base + j < end ? weight(x[j], base + j) : 0, sum += w[j];
-    u64 b = before + wave_before(sum);
-    const bool hit = b <= goal && goal < b + sum;
-    if (hit) {
-      bool done = false;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (!done && goal < b + w[j]) {
-          g.ids[row] = base + j;
-          g.prob[row] = static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total));
-          done = true;
-        }
-        b += w[j];
-      }
+    for (int j = 0; j < V; ++j) w[j] = base + j < end ? kept(x[j], base + j, sc, limit, r.m) : 0;
+    if (draw<V>(g, row, base, w, goal, total, before)) return;
+  }
+}
+
+// items a workgroup holds in registers
+constexpr int kRowItems = 16384;
+
+// long rows: the workspace, from `base` on (null: its size alone)
+inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* base) {
+  const int64_t vec = 16 / size;
+  g.span = static_cast<int>(4 * kWave * vec);            // four vectors a lane
+  while ((n + g.span - 1) / g.span > kChunks) g.span *= 2;
+  g.chunks = static_cast<int>((n + g.span - 1) / g.span);
+  // enough pieces for four workgroups a compute unit, of at least 8192 items
+  const int64_t want = std::min<int64_t>({kMaxPieces, std::max<int64_t>(1, 1024 / rows), std::max<int64_t>(1, n / 8192)});
+  const int64_t per = (g.chunks + want - 1) / want;
+  g.piece = static_cast<int>(std::min<int64_t>(per * g.span, int64_t{1} << 30));
+  g.pieces = static_cast<int>((g.chunks + per - 1) / per);
+  g.room = std::max(1024, g.piece / 8);
+  size_t at = 0;
+  auto take = [&](auto*& p, size_t count) {
+    p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
+    at += (count * sizeof(*p) + 255) & ~size_t{255};
+  };
+  const size_t all = static_cast<size_t>(rows) * g.pieces;
+  take(g.tops, all);
+  take(g.mass, all * kBins);
+  take(g.count, all * kBins);
+  take(g.state, rows);
+  take(g.listed, all);
+  take(g.list, all * g.room);
+  take(g.chunk, static_cast<size_t>(rows) * g.chunks);
+  return at;
+}
+
+template <typename T>
+void launch(const SampleArgs& g, bool limits, hipStream_t st) {
+  const dim3 rows(static_cast<unsigned>(g.rows)), block(kThreads);
+  constexpr int V = 16 / sizeof(T);
+  if (g.n <= kThreads * V) {
+    hipLaunchKernelGGL((sample_row_kernel<T, 1>), rows, block, 0, st, g);
+  } else if (g.n <= 2 * kThreads * V) {
+    hipLaunchKernelGGL((sample_row_kernel<T, 2>), rows, block, 0, st, g);
+  } else if (g.n <= kRowItems) {
+    if constexpr (V == 4) hipLaunchKernelGGL((sample_row_kernel<T, 4>), rows, block, 0, st, g);
+  } else {
+    const dim3 pieces(static_cast<unsigned>(g.rows) * g.pieces);
+    hipLaunchKernelGGL(sample_top_kernel<T>, pieces, dim3(256), 0, st, g);
+    if (limits) {
+      hipLaunchKernelGGL(sample_histogram_kernel<T>, pieces, block, 0, st, g);
+      hipLaunchKernelGGL(sample_bins_kernel, rows, block, 0, st, g);
     }
-    if (__ballot(hit)) return;
-    before += wave_sum(sum);
+    hipLaunchKernelGGL(sample_pieces_kernel<T>, pieces, dim3(256), 0, st, g);
+    hipLaunchKernelGGL(sample_draw_kernel<T>, rows, block, 0, st, g);
   }
 }
 
@@ -363,16 +724,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs g) {
 
 using namespace sg;
 
-SG_API size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n) {
-  (void)rows, (void)n;
-  return 0;
+SG_API size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n, int dtype) {
+  if (rows <= 0 || n <= kRowItems || n >= SG_SAMPLE_MAX_ITEMS || !valid_dtype(dtype)) return 0;
+  SampleArgs g{};
+  return lay_out(g, rows, n, dtype == SG_DTYPE_F32 ? 4 : 2, nullptr);
 }
 
 SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld, int dtype, const float* u, int64_t rows,
                               int64_t n, double temperature, int64_t top_k, double top_p, double min_p, const float* temperature_rows,
                               const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, void* workspace,
                               size_t workspace_bytes, void* stream) {
-  (void)workspace, (void)workspace_bytes;
   if (!valid_dtype(dtype)) return fail(SG_ERR_INVALID, "sample_rows: unknown dtype %d", dtype);
   if (rows < 0 || n < 0) return fail(SG_ERR_INVALID, "sample_rows: negative size");
   if (rows >= (1ll << 31) || n >= SG_SAMPLE_MAX_ITEMS) return fail(SG_ERR_UNSUPPORTED, "sample_rows: fewer than %d items", SG_SAMPLE_MAX_ITEMS);
@@ -381,14 +742,23 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
   if (ld < n) return fail(SG_ERR_INVALID, "sample_rows: rows overlap");
   if (!(temperature >= 0.0) || !(top_p >= 0.0) || !(min_p >= 0.0) || top_k < 0)
     return fail(SG_ERR_INVALID, "sample_rows: temperature, top_k, top_p and min_p must not be negative");
+  if (n > kRowItems && rows * kMaxPieces >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
+  if (workspace_bytes < sg_sample_rows_workspace_bytes(rows, n, dtype) || (n > kRowItems && !workspace))
+    return fail(SG_ERR_WORKSPACE, "sample_rows workspace too small");
   int log_n = 0;
   while ((1ll << log_n) < n) ++log_n;
-  SampleArgs g{ids, prob, logits, u, temperature_rows, top_k_rows, top_p_rows, min_p_rows, temperature, top_p, min_p, ld, top_k,
-               static_cast<int>(rows), static_cast<int>(n), std::min(51, 62 - log_n)};
+  SampleArgs g{};
+  g.ids = ids, g.prob = prob, g.l = logits, g.u = u;
+  g.temperature = temperature_rows, g.top_k = top_k_rows, g.top_p = top_p_rows, g.min_p = min_p_rows;
+  g.t0 = temperature, g.p0 = top_p, g.m0 = min_p, g.k0 = top_k;
+  g.ld = ld, g.rows = static_cast<int>(rows), g.n = static_cast<int>(n), g.bits = std::min(51, 62 - log_n);
+  if (n > kRowItems) lay_out(g, rows, n, dtype == SG_DTYPE_F32 ? 4 : 2, static_cast<char*>(workspace));
+  // whether any row can have a limit: otherwise the histogram has no reader
+  const bool limits = top_k_rows || top_p_rows || temperature_rows || min_p_rows || (top_k > 0 && top_k < n) || top_p < 1.0 ||
+                      temperature == 0.0 || min_p > 1.0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(rows));
-  if (dtype == SG_DTYPE_F32) hipLaunchKernelGGL(sample_kernel<float>, grid, dim3(kThreads), 0, st, g);
-  else if (dtype == SG_DTYPE_F16) hipLaunchKernelGGL(sample_kernel<f16>, grid, dim3(kThreads), 0, st, g);
-  else hipLaunchKernelGGL(sample_kernel<bf16>, grid, dim3(kThreads), 0, st, g);
+  if (dtype == SG_DTYPE_F32) launch<float>(g, limits, st);
+  else if (dtype == SG_DTYPE_F16) launch<f16>(g, limits, st);
+  else launch<bf16>(g, limits, st);
   return check_launch("sample_rows");
 }

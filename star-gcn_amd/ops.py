@@ -555,7 +555,7 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     ids = torch.empty((rows,), dtype=torch.int32, device=logits.device)
     prob = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     lib = L.lib()
-    wsn = lib.sg_sample_rows_workspace_bytes(rows, n)
+    wsn = lib.sg_sample_rows_workspace_bytes(rows, n, dt)
     ws = L.scratch(wsn, logits.device)
     L.check(lib.sg_sample_rows_hip(L.ptr(ids), L.ptr(prob), L.ptr(logits), ld, dt, L.ptr(u), rows, n, float(t), int(k), float(p),
                                    float(m), L.ptr(tr), L.ptr(kr), L.ptr(pr), L.ptr(mr), L.ptr(ws), wsn, L.stream_ptr()),

@@ -64,7 +64,7 @@ def test_split_products_and_long_rows_ask_for_their_workspace():
     assert gemm(M=64, N=64, K=8192, lda=8192, ldb=8192, ldc=64) == -5
     assert gemm(M=64, N=64, K=8192, lda=8192, ldb=8192, ldc=64, ws=P, wsn=need - 1) == -5
     assert lib.sg_gemm_i8_workspace_bytes(0, 64, 8192) == 0
-    need = lib.sg_sample_rows_workspace_bytes(1, 1000000)
+    need = lib.sg_sample_rows_workspace_bytes(1, 1000000, 0)
     if need:
         assert sample(rows=1, n=1000000, ld=1000000, wsn=need - 1) == -5 and sample(rows=1, n=1000000, ld=1000000, ws=None, wsn=0) == -5
 
