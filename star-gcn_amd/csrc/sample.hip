@@ -17,10 +17,12 @@
 //
 // Rows of up to 16384 items: one workgroup a row, the row in its registers.  Longer rows are cut into pieces, five launches:
 // maximum; histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits
-// and draw.  A list that overflows (many equal scores) is replaced by passes over the row.
+// and draw.  A list of more than 8192
+// candidates (many equal scores) is replaced by passes over the row.
 #include "rows_shared.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sg {
 namespace {
@@ -29,6 +31,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 constexpr int kBins = 2048;        // of the histogram and of a subdivision: two a thread
 constexpr int kFew = 512;          // candidates that are ranked against each other
 constexpr int kChunks = 4096;      // partial weights by index of a long row
+constexpr int kListed = 8192;      // candidates of a long row's limits
 constexpr int kMaxPieces = 32;
 
 typedef unsigned long long u64;
@@ -90,49 +93,46 @@ __device__ __forceinline__ float score_at(u64 place) {
 }
 __device__ __forceinline__ int index_at(u64 place) { return static_cast<int>(~static_cast<unsigned>(place)); }
 
-// d = (max - l) log2(e) / T, >= 0; NaN and -inf: beyond every weight
-__device__ __forceinline__ double below_top(float l, float top, double c) {
-  if (l == top) return 0.0;
-  const double d = (static_cast<double>(top) - static_cast<double>(l)) * c;
-  return d >= 0.0 ? d : __builtin_inf();
-}
-
-// 2^(bits - d), rounded to a whole number by the caller (Taylor series of 2^f, |f| <= 1/2: the first term left out is 6e-15)
-__device__ __forceinline__ double scaled_weight(double d, int bits) {
-  if (!(d < bits + 1.0)) return 0.0;
-  const double n = rint(d), f = n - d;
-  double y = 4.44553827187081e-10;                       // (ln 2)^11 / 11!
-  y = fma(y, f, 7.054911620801121e-09);
-  y = fma(y, f, 1.0178086009239696e-07);
-  y = fma(y, f, 1.3215486790144305e-06);
-  y = fma(y, f, 1.5252733804059838e-05);
-  y = fma(y, f, 0.00015403530393381606);
-  y = fma(y, f, 0.0013333558146428441);
-  y = fma(y, f, 0.009618129107628477);
-  y = fma(y, f, 0.055504108664821576);
-  y = fma(y, f, 0.2402265069591007);
-  y = fma(y, f, 0.6931471805599453);
-  y = fma(y, f, 1.0);
-  return ldexp(y, bits - static_cast<int>(n));
-}
-__device__ __forceinline__ u64 whole(double w) {              // w < 2^52
-  return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) - 0x4330000000000000ull;
-}
-
-__device__ __forceinline__ int bin_of(double d, double scale) { return static_cast<int>(fmin(d * scale, kBins - 1.0)); }
-
-
-// a row's scale: what turns a score into a bin and a weight
+// A row's scale: what turns a score into a bin of the histogram and into a weight.  d = (max - l) log2(e) / T; an item is live
+// if d < last: -inf, NaN and what lies so far below that its weight is 0 are not.  In the bit patterns: adding 1.5 * 2^52 to a
+// double rounds it to a whole number that stands in its low bits, for a quarter of a conversion's cost.
 struct Scale {
-  float top;
-  double c, bins;
+  double top, c, last, bins;
   int bits;
-  __device__ __forceinline__ double below(float l) const { return below_top(l, top, c); }
-  __device__ __forceinline__ int bin(double d) const { return bin_of(d, bins); }
-  __device__ __forceinline__ double weight(double d) const { return scaled_weight(d, bits); }
+  bool endless;                    // max = +inf: only the items that equal it are live
+
+  __device__ __forceinline__ double below(float l) const {
+    const double d = (top - static_cast<double>(l)) * c;
+    return endless ? (static_cast<double>(l) == top ? 0.0 : 2.0 * last) : d;
+  }
+  __device__ __forceinline__ bool live(double d) const { return d < last; }
+  // of a live item: 0 .. kBins - 2
+  __device__ __forceinline__ int bin(double d) const {
+    return static_cast<int>(static_cast<unsigned>(__double_as_longlong(fma(d, bins, 6755399441055744.0))));
+  }
+  // of a live item: 2^(bits - d), to be rounded to a whole number.  2^f for |f| <= 1/2 by 1 + f times a polynomial that
+  // interpolates (2^f - 1) / f at Chebyshev's points: 4e-14, and exact at f = 0
+  __device__ __forceinline__ double weight(double d) const {
+    const double t = d + 6755399441055744.0, f = (t - 6755399441055744.0) - d;
+    double y = 1.0203121047189341e-07;
+    y = fma(y, f, 1.3255224879317324e-06);
+    y = fma(y, f, 1.525268684635191e-05);
+    y = fma(y, f, 0.0001540345585244999);
+    y = fma(y, f, 0.0013333558179042969);
+    y = fma(y, f, 0.009618129159402565);
+    y = fma(y, f, 0.055504108664760424);
+    y = fma(y, f, 0.2402265069581299);
+    y = fma(y, f, 0.6931471805599453);
+    y = fma(y, f, 1.0);
+    const int n = static_cast<int>(static_cast<unsigned>(__double_as_longlong(t)));
+    return __hiloint2double(__double2hiint(y) + (bits - n) * (1 << 20), __double2loint(y));
+  }
 };
 __device__ __forceinline__ Scale scale_of(float top, const Row& r, int bits) {
-  return Scale{top, r.c, (kBins - 1.0) / (bits + 1.0), bits};      // the last bin holds items of weight 0 only
+  return Scale{top, r.c, bits + 1.0, (kBins - 2.0) / (bits + 1.0), bits, top == __builtin_inff()};
+}
+__device__ __forceinline__ u64 whole(double w) {                  // w < 2^52, to the nearest
+  return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
 struct Histogram {
@@ -192,15 +192,14 @@ __device__ __forceinline__ void clear(Histogram& h) {
 }
 
 template <typename Src>
-__device__ __forceinline__ void fill(Histogram& h, const Src& src, const Scale& sc, bool masses) {
+__device__ __forceinline__ void fill(Histogram& h, const Src& src, const Scale& sc, bool counts, bool masses) {
   clear(h);
   src([&](float l, int) {
     const double d = sc.below(l);
-    if (d == __builtin_inf()) return;
+    if (!sc.live(d)) return;
     const int b = sc.bin(d);
-    atomicAdd(&h.count[b], 1u);
-    const u64 w = masses ? whole(sc.weight(d)) : 0;
-    if (w) atomicAdd(&h.mass[b], w);
+    if (counts) atomicAdd(&h.count[b], 1u);
+    if (masses) atomicAdd(&h.mass[b], whole(sc.weight(d)));
   });
   __syncthreads();
 }
@@ -222,68 +221,68 @@ __device__ __forceinline__ u64 share(double p, u64 total) {        // the weight
   return min(max(need, u64{1}), total);
 }
 
-// The limit among the n items of `src` in bins lo_bin .. hi_bin, before which `count` items of weight `mass` stand in the order:
-// by count, the item with which the count reaches `need`; by mass, the item with which the weight does.  -> its place; mass:
-// with the item itself.
+// The limit among the live items of `src` in bins lo_bin .. hi_bin, before which `count` items of weight `mass` stand in the
+// order: by count, the item with which the count reaches `need`; by mass, the item with which the weight does.  -> its place;
+// mass: with the item itself (by count only where `masses`).
 template <typename Src>
-__device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, unsigned n, bool by_mass,
+__device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, bool by_mass, bool masses,
                                           u64 need, unsigned count, u64& mass) {
   const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
   u64 lo = 0, hi = ~u64{0};
   auto members = [&](auto f) {
     src([&](float l, int i) {
       const double d = sc.below(l);
-      if (d == __builtin_inf()) return;
+      if (!sc.live(d)) return;
       const int b = sc.bin(d);
       if (b < lo_bin || b > hi_bin) return;
       const u64 at = place(l, i);
       if (at >= lo && at <= hi) f(at, d);
     });
   };
-  if (n > kFew) {                                        // the range they span
-    u64 least = ~u64{0}, most = 0;
-    members([&](u64 at, double) { least = min(least, at), most = max(most, at); });
-    for (int off = 32; off > 0; off >>= 1) {
-      least = min(least, static_cast<u64>(__shfl_xor(least, off)));
-      most = max(most, static_cast<u64>(__shfl_xor(most, off)));
-    }
-    if (lane == 0) sh.wave_a[wave] = least, sh.wave_b[wave] = most;
+  for (bool first = true;; first = false) {
+    if (t == 0) sh.few = 0, sh.limit = lo, sh.limit_mass = mass;
     __syncthreads();
-    lo = sh.wave_a[0], hi = sh.wave_b[0];
-    for (int i = 1; i < kWaves; ++i) lo = min(lo, sh.wave_a[i]), hi = max(hi, sh.wave_b[i]);
-  }
-  while (n > kFew) {                                     // all places differ: every turn leaves at most 1 / 2048 of the range
+    members([&](u64 at, double d) {
+      const unsigned k = atomicAdd(&sh.few, 1u);
+      if (k < kFew) sh.few_place[k] = at, sh.few_weight[k] = masses ? whole(sc.weight(d)) : 0;
+    });
+    __syncthreads();
+    if (sh.few <= kFew) break;
+    if (first) {                                         // the range they span
+      u64 least = ~u64{0}, most = 0;
+      members([&](u64 at, double) { least = min(least, at), most = max(most, at); });
+      for (int off = 32; off > 0; off >>= 1) {
+        least = min(least, static_cast<u64>(__shfl_xor(least, off)));
+        most = max(most, static_cast<u64>(__shfl_xor(most, off)));
+      }
+      if (lane == 0) sh.wave_a[wave] = least, sh.wave_b[wave] = most;
+      __syncthreads();
+      lo = sh.wave_a[0], hi = sh.wave_b[0];
+      for (int i = 1; i < kWaves; ++i) lo = min(lo, sh.wave_a[i]), hi = max(hi, sh.wave_b[i]);
+    }
+    // all places differ: a turn leaves at most 1 / 1024 of the range, and single places at last
     const int shift = max(0, 53 - __clzll(static_cast<long long>(hi - lo)));
     clear(sh.sub);
     members([&](u64 at, double d) {
       const int digit = static_cast<int>((hi - at) >> shift);
-      atomicAdd(&sh.sub.count[digit], 1u);
-      const u64 w = whole(sc.weight(d));
-      if (w) atomicAdd(&sh.sub.mass[digit], w);
+      if (!by_mass) atomicAdd(&sh.sub.count[digit], 1u);
+      if (masses) atomicAdd(&sh.sub.mass[digit], whole(sc.weight(d)));
     });
     __syncthreads();
     unsigned bc;
     u64 bm;
     const int digit = min(find_bin(sh, sh.sub, by_mass, need - (by_mass ? mass : count), bc, bm), kBins - 1);
-    n = sh.sub.count[digit];
     count += bc, mass += bm;
     hi -= static_cast<u64>(digit) << shift;
     lo = max(lo, hi - ((u64{1} << shift) - 1));
-    __syncthreads();
   }
-  if (t == 0) sh.few = 0, sh.limit = lo, sh.limit_mass = mass;
-  __syncthreads();
-  members([&](u64 at, double d) {
-    const unsigned k = atomicAdd(&sh.few, 1u);
-    if (k < kFew) sh.few_place[k] = at, sh.few_weight[k] = whole(sc.weight(d));
-  });
-  __syncthreads();
   // each against all: `team` threads a candidate
-  const int m = min(static_cast<int>(sh.few), kFew);
+  const int m = static_cast<int>(sh.few);
   int team = kWave;
   while (team * m > kThreads) team >>= 1;
   const int me = t / team;
-  u64 cb = 0, mb = 0;
+  u64 mb = 0;
+  unsigned cb = 0;
   const u64 at = me < m ? sh.few_place[me] : 0;
   if (me < m)
     for (int j = t % team; j < m; j += team)
@@ -303,7 +302,7 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
 // the weight of an item if it is kept: its place is not below `limit`, the lower of the limits
 __device__ __forceinline__ u64 kept(float l, int i, const Scale& sc, u64 limit, double min_weight) {
   const double d = sc.below(l);
-  if (!(d < sc.bits + 1.0) || place(l, i) < limit) return 0;
+  if (!sc.live(d) || place(l, i) < limit) return 0;
   const double w = sc.weight(d);
   return w >= min_weight ? whole(w) : 0;
 }
@@ -385,20 +384,20 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
   };
   u64 limit = 0;
   if (r.k > 0 || r.by_p) {
-    fill(hist, src, sc, r.by_p);
+    fill(hist, src, sc, r.k > 0, r.by_p);
     unsigned count;
     u64 mass, total = r.by_p ? total_mass(sh, hist) : 0;
     if (r.k > 0) {
       const int b = find_bin(sh, hist, false, static_cast<u64>(r.k), count, mass);
-      if (b < kBins - 1) {
-        limit = find_limit(sh, src, sc, b, b, hist.count[b], false, static_cast<u64>(r.k), count, mass);
+      if (b < kBins) {
+        limit = find_limit(sh, src, sc, b, b, false, r.by_p, static_cast<u64>(r.k), count, mass);
         total = mass;
       }
     }
     if (r.by_p) {
       const u64 need = share(r.p, total);
       const int b = find_bin(sh, hist, true, need, count, mass);
-      if (b < kBins - 1) limit = max(limit, find_limit(sh, src, sc, b, b, hist.count[b], true, need, count, mass));
+      if (b < kBins) limit = max(limit, find_limit(sh, src, sc, b, b, true, true, need, count, mass));
     }
   }
   // kept weight by index: level i of wave w comes after level i of wave w - 1, and after every wave's level i - 1
@@ -432,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
 
 struct RowState {
   u64 total, k_mass, p_mass;       // weight of the row; before the top-k bin; before the top-p bins
-  unsigned k_count, k_items, p_items;      // items before the top-k bin, in it, in the top-p bins
+  unsigned k_count;                // items before the top-k bin
   int k_bin, p_lo, p_hi;           // kBins: no such limit
 };
 
@@ -476,10 +475,13 @@ __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const Sample
   const Row r = row_settings(g, row);
   if (!(r.k > 0 || r.by_p)) return;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
-  fill(hist, [&](auto f) { each(l, lo, hi, f); }, scale_of(row_top(g, row), r, g.bits), r.by_p || r.k > 0);
+  fill(hist, [&](auto f) { each(l, lo, hi, f); }, scale_of(row_top(g, row), r, g.bits), r.k > 0, r.by_p);
   u64* mass = g.mass + static_cast<long long>(blockIdx.x) * kBins;
   unsigned* count = g.count + static_cast<long long>(blockIdx.x) * kBins;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = hist.mass[i], count[i] = hist.count[i];
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    if (r.by_p) mass[i] = hist.mass[i];
+    if (r.k > 0) count[i] = hist.count[i];
+  }
 }
 
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs g) {
@@ -487,38 +489,35 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   __shared__ Histogram hist;
   const int row = blockIdx.x, t = threadIdx.x;
   const Row r = row_settings(g, row);
-  RowState s{0, 0, 0, 0, 0, 0, kBins, kBins, kBins};
+  RowState s{0, 0, 0, 0, kBins, kBins, kBins};
   if (r.k > 0 || r.by_p) {
-    for (int i = t; i < kBins; i += kThreads) {
-      u64 m = 0;
-      unsigned c = 0;
-      for (int z = 0; z < g.pieces; ++z) {
-        const long long at = (static_cast<long long>(row) * g.pieces + z) * kBins + i;
-        m += g.mass[at], c += g.count[at];
+    const long long at = static_cast<long long>(row) * g.pieces * kBins + 2 * t;      // this thread's two bins
+    u64 m0 = 0, m1 = 0;
+    unsigned c0 = 0, c1 = 0;
+#pragma unroll 8
+    for (int z = 0; z < g.pieces; ++z) {
+      if (r.by_p) {
+        const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(g.mass + at + static_cast<long long>(z) * kBins);
+        m0 += m.x, m1 += m.y;
       }
-      hist.mass[i] = m, hist.count[i] = c;
+      if (r.k > 0) {
+        const uint2 c = *reinterpret_cast<const uint2*>(g.count + at + static_cast<long long>(z) * kBins);
+        c0 += c.x, c1 += c.y;
+      }
     }
+    hist.mass[2 * t] = m0, hist.mass[2 * t + 1] = m1, hist.count[2 * t] = c0, hist.count[2 * t + 1] = c1;
     __syncthreads();
-    s.total = total_mass(sh, hist);
-    u64 least = s.total, most = s.total;                 // weight of the top-k items
+    u64 most = 0, least = 0;                             // the weight of the top-k items lies between them
+    if (r.by_p) least = most = s.total = total_mass(sh, hist);
     if (r.k > 0) {
-      const int b = find_bin(sh, hist, false, static_cast<u64>(r.k), s.k_count, s.k_mass);
-      if (b < kBins - 1) s.k_bin = b, s.k_items = hist.count[b], least = s.k_mass, most = s.k_mass + hist.mass[b];
+      s.k_bin = find_bin(sh, hist, false, static_cast<u64>(r.k), s.k_count, s.k_mass);
+      if (s.k_bin < kBins) least = s.k_mass, most = s.k_mass + hist.mass[s.k_bin];
     }
-    if (r.by_p && s.total > 0) {                         // total = 0: a row of nothing but -inf and NaN
+    if (r.by_p && s.total > 0) {                         // no total: a row of nothing but -inf and NaN
       unsigned c;
       u64 m;
       s.p_hi = find_bin(sh, hist, true, share(r.p, most), c, m);
-      s.p_hi = min(s.p_hi, kBins - 1);
-      s.p_lo = least > 0 ? min(find_bin(sh, hist, true, share(r.p, least), c, s.p_mass), s.p_hi) : 0;
-      if (least == 0) s.p_mass = 0;
-      u64 items = 0;
-      for (int i = t; i < kBins; i += kThreads)
-        if (i >= s.p_lo && i <= s.p_hi) items += hist.count[i];
-      items = wave_sum(items);
-      if (t % kWave == 0) sh.wave_a[t / kWave] = items;
-      __syncthreads();
-      for (int i = 0; i < kWaves; ++i) s.p_items += static_cast<unsigned>(sh.wave_a[i]);
+      s.p_lo = least > 0 ? find_bin(sh, hist, true, share(r.p, least), c, s.p_mass) : 0;
     }
   }
   if (t == 0) g.state[row] = s;
@@ -536,7 +535,7 @@ __global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) 
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   const Row r = row_settings(g, row);
   const Scale sc = scale_of(row_top(g, row), r, g.bits);
-  RowState s{0, 0, 0, 0, 0, 0, kBins, kBins, kBins};
+  RowState s{0, 0, 0, 0, kBins, kBins, kBins};
   if (r.k > 0 || r.by_p) s = g.state[row];
   u64* list = g.list + static_cast<long long>(blockIdx.x) * g.room;
   if (threadIdx.x == 0) listed = 0;
@@ -554,8 +553,8 @@ __global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) 
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const int i = base + u * kWave * V + j;
-          const double d = i < end ? sc.below(x[u][j]) : __builtin_inf();
-          if (!(d < sc.bits + 1.0)) continue;
+          const double d = sc.below(x[u][j]);
+          if (i >= end || !sc.live(d)) continue;
           const int b = sc.bin(d);
           if (surely_kept(s, b)) {
             const double w = sc.weight(d);
@@ -576,7 +575,7 @@ __global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs g) {
   __shared__ Shared sh;
-  __shared__ u64 chunk[kChunks];
+  __shared__ u64 chunk[kChunks], lds_list[kListed];
   constexpr int V = 16 / sizeof(T);
   const int row = blockIdx.x, t = threadIdx.x, wave = t / kWave, lane = t % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
@@ -587,37 +586,44 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     return;
   }
   const Scale sc = scale_of(top, r, g.bits);
-  RowState s{0, 0, 0, 0, 0, 0, kBins, kBins, kBins};
+  RowState s{0, 0, 0, 0, kBins, kBins, kBins};
   if (r.k > 0 || r.by_p) s = g.state[row];
   for (int i = t; i < g.chunks; i += kThreads) chunk[i] = g.chunk[static_cast<long long>(row) * g.chunks + i];
   u64 limit = 0;
   if (s.k_bin < kBins || s.p_lo < kBins) {
+    // the pieces' lists, one behind the other in LDS if they fit
+    int listed = 0;
     bool whole_list = true;
-    for (int z = 0; z < g.pieces; ++z) whole_list = whole_list && g.listed[row * g.pieces + z] <= static_cast<unsigned>(g.room);
+    for (int z = 0; z < g.pieces; ++z) {
+      const unsigned n = g.listed[row * g.pieces + z];
+      whole_list = whole_list && n <= static_cast<unsigned>(g.room);
+      if (!whole_list) break;
+      if (z % kWaves == wave)
+        for (int i = lane; i < static_cast<int>(n) && listed + i < kListed; i += kWave)
+          lds_list[listed + i] = g.list[(static_cast<long long>(row) * g.pieces + z) * g.room + i];
+      listed += static_cast<int>(n);
+    }
+    whole_list = whole_list && listed <= kListed;
     auto limits = [&](auto src) {
       u64 mass = s.k_mass, total = s.total;
       if (s.k_bin < kBins) {
-        limit = find_limit(sh, src, sc, s.k_bin, s.k_bin, s.k_items, false, static_cast<u64>(r.k), s.k_count, mass);
+        limit = find_limit(sh, src, sc, s.k_bin, s.k_bin, false, r.by_p, static_cast<u64>(r.k), s.k_count, mass);
         total = mass;
       }
       if (s.p_lo < kBins) {
         mass = s.p_mass;
-        limit = max(limit, find_limit(sh, src, sc, s.p_lo, s.p_hi, s.p_items, true, share(r.p, total), 0, mass));
+        limit = max(limit, find_limit(sh, src, sc, s.p_lo, s.p_hi, true, true, share(r.p, total), 0, mass));
       }
     };
     if (whole_list) {
       auto src = [&](auto f) {
-        for (int z = 0; z < g.pieces; ++z) {
-          const u64* list = g.list + (static_cast<long long>(row) * g.pieces + z) * g.room;
-          const int n = static_cast<int>(g.listed[row * g.pieces + z]);
-          for (int i = t; i < n; i += kThreads) {
-            const u64 at = list[i];
-            f(score_at(at), index_at(at));
-          }
+        for (int i = t; i < listed; i += kThreads) {
+          const u64 at = lds_list[i];
+          f(score_at(at), index_at(at));
         }
       };
-      limits(src);
       __syncthreads();
+      limits(src);
       src([&](float x, int i) {
         const u64 w = kept(x, i, sc, limit, r.m);
         if (w) atomicAdd(&chunk[i / g.span], w);
@@ -680,7 +686,7 @@ inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* ba
   const int64_t per = (g.chunks + want - 1) / want;
   g.piece = static_cast<int>(std::min<int64_t>(per * g.span, int64_t{1} << 30));
   g.pieces = static_cast<int>((g.chunks + per - 1) / per);
-  g.room = std::max(1024, g.piece / 8);
+  g.room = std::min(kListed, g.piece / 4);
   size_t at = 0;
   auto take = [&](auto*& p, size_t count) {
     p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
