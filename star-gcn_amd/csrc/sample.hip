@@ -15,10 +15,11 @@
 // the order (score and index in 64 bits, all different) until they are.  -inf and NaN are scores of items that are never drawn;
 // a row without any other draws -1.
 //
-// Rows of up to 16384 items: one workgroup a row, the row in its registers.  Longer rows are cut into pieces, five launches:
-// maximum; histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits
-// and draw.  A list of more than 8192
-// candidates (many equal scores) is replaced by passes over the row.
+// Rows of up to 16384 items: one workgroup a row, the row in LDS.  Longer rows are cut into pieces, five launches: maximum;
+// histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits and draw.
+// A list of more than 8192 candidates (many equal scores) is replaced by passes over the row.  64 rows of 1,000,000 fp32 scores,
+// top-p: 36 us for the maximum (6.9 TB/s), 88 for the histogram (bound by the 64-bit arithmetic and its LDS additions), 9, 62
+// and 9 for the rest.
 #include "rows_shared.hpp"
 
 #include <algorithm>
@@ -27,12 +28,15 @@
 namespace sg {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / kWave;
-constexpr int kBins = 2048;        // of the histogram and of a subdivision: two a thread
+// 512 threads and up to 128 registers: two workgroups a compute unit (512 rows of 10677: 31 us; of 1024 threads, one at a time: 43)
+constexpr int kThreads = 512, kWaves = kThreads / kWave;
+constexpr int kBins = 2048;        // of the histogram and of a subdivision
+constexpr int kPer = kBins / kThreads;
 constexpr int kFew = 512;          // candidates that are ranked against each other
 constexpr int kChunks = 4096;      // partial weights by index of a long row
 constexpr int kListed = 8192;      // candidates of a long row's limits
 constexpr int kMaxPieces = 32;
+constexpr int kLevels = 4096 / kThreads;      // groups of four that a thread holds of a short row
 
 typedef unsigned long long u64;
 
@@ -66,6 +70,16 @@ struct Row {                       // a row's settings, the same on every thread
   bool by_p;
 };
 
+// a value that every lane holds, into scalar registers: what a row is scaled and compared with would fill a third of the vector
+// registers
+__device__ __forceinline__ u64 uniform(u64 v) {
+  return static_cast<u64>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32)))) << 32 |
+         static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+}
+__device__ __forceinline__ double uniform(double v) {
+  return __longlong_as_double(static_cast<long long>(uniform(static_cast<u64>(__double_as_longlong(v)))));
+}
+
 __device__ __forceinline__ Row row_settings(const SampleArgs& g, int row) {
   Row r;
   const double t = g.temperature ? g.temperature[row] : g.t0;
@@ -76,8 +90,8 @@ __device__ __forceinline__ Row row_settings(const SampleArgs& g, int row) {
   r.by_p = !(r.p >= 1.0);
   if (!(t > 0.0) || !(r.p > 0.0) || !(m <= 1.0)) r.k = 1;      // nothing but the first item
   if (r.k == 1) r.by_p = false, m = 0.0;
-  r.c = t > 0.0 ? 1.4426950408889634074 / t : 1.0;
-  r.m = m > 0.0 ? ldexp(m, g.bits) : 0.0;
+  r.c = uniform(t > 0.0 ? 1.4426950408889634074 / t : 1.0);
+  r.m = uniform(m > 0.0 ? ldexp(m, g.bits) : 0.0);
   return r;
 }
 
@@ -129,7 +143,8 @@ struct Scale {
   }
 };
 __device__ __forceinline__ Scale scale_of(float top, const Row& r, int bits) {
-  return Scale{top, r.c, bits + 1.0, (kBins - 2.0) / (bits + 1.0), bits, top == __builtin_inff()};
+  return Scale{uniform(static_cast<double>(top)), r.c, uniform(bits + 1.0), uniform((kBins - 2.0) / (bits + 1.0)), bits,
+               top == __builtin_inff()};
 }
 __device__ __forceinline__ u64 whole(double w) {                  // w < 2^52, to the nearest
   return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
@@ -141,7 +156,8 @@ struct Histogram {
 };
 
 struct Shared {
-  Histogram sub;                   // of a subdivision
+  Histogram hist;                  // of the row, or of a subdivision
+  bool divided;                    // a subdivision has replaced the row's
   u64 few_place[kFew], few_weight[kFew];
   u64 wave_a[kWaves], wave_b[kWaves];
   u64 before_mass, limit, limit_mass;
@@ -149,39 +165,53 @@ struct Shared {
   int found;
 };
 
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+// Sum of the lanes up to this one.  On the vector ALU (shifts inside rows of 16 lanes, then lanes 15 and 31 into the rows behind
+// them): a shuffle through LDS costs a hundred cycles a step.
+__device__ __forceinline__ u64 wave_upto(u64 v) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), C, R, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), C, R, 0xf, false);
+    v += static_cast<u64>(hi) << 32 | lo;
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});      // row_shr:1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});      // row_bcast:15 into rows 1 and 3
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});      // row_bcast:31 into rows 2 and 3
   return v;
 }
-
-// sums of all lanes below this one
-__device__ __forceinline__ u64 wave_before(u64 v) {
-  const int lane = threadIdx.x % kWave;
-  u64 s = v;
-  for (int off = 1; off < kWave; off <<= 1) {
-    const u64 o = __shfl_up(s, off);
-    if (lane >= off) s += o;
-  }
-  return s - v;
+__device__ __forceinline__ u64 from_lane(u64 v, int lane) {
+  return static_cast<u64>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+         static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
+__device__ __forceinline__ u64 wave_sum(u64 v) { return from_lane(wave_upto(v), kWave - 1); }
+__device__ __forceinline__ u64 wave_before(u64 v) { return wave_upto(v) - v; }      // sum of the lanes below this one
 
 // The bin, counted from bin 0 on, in which the sum of counts reaches `need` (by_mass: the sum of weights), and the sums before
-// it; kBins if there is none.  Two bins a thread.
+// it; kBins if there is none.
 __device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, bool by_mass, u64 need, unsigned& before_count, u64& before_mass) {
-  const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   if (t == 0) sh.found = kBins, sh.before_count = 0, sh.before_mass = 0;
-  const u64 m0 = h.mass[2 * t], m1 = h.mass[2 * t + 1];
-  const unsigned c0 = h.count[2 * t], c1 = h.count[2 * t + 1];
-  u64 mb = wave_before(m0 + m1), cb = wave_before(static_cast<u64>(c0) + c1);
-  if (lane == kWave - 1) sh.wave_a[wave] = mb + m0 + m1, sh.wave_b[wave] = cb + c0 + c1;
+  u64 m[kPer], ms = 0;
+  unsigned c[kPer], cs = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) m[i] = h.mass[kPer * t + i], c[i] = h.count[kPer * t + i], ms += m[i], cs += c[i];
+  u64 mb = wave_before(ms), cb = wave_before(cs);
+  if (lane == kWave - 1) sh.wave_a[wave] = mb + ms, sh.wave_b[wave] = cb + cs;
   __syncthreads();
   for (int i = 0; i < wave; ++i) mb += sh.wave_a[i], cb += sh.wave_b[i];
-  const u64 a = by_mass ? mb : cb, v0 = by_mass ? m0 : c0, v1 = by_mass ? m1 : c1;
-  if (a < need && need <= a + v0) sh.found = 2 * t, sh.before_count = static_cast<unsigned>(cb), sh.before_mass = mb;
-  else if (a + v0 < need && need <= a + v0 + v1) sh.found = 2 * t + 1, sh.before_count = static_cast<unsigned>(cb) + c0, sh.before_mass = mb + m0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const u64 a = by_mass ? mb : cb, v = by_mass ? m[i] : c[i];
+    if (a < need && need <= a + v) sh.found = kPer * t + i, sh.before_count = static_cast<unsigned>(cb), sh.before_mass = mb;
+    mb += m[i], cb += c[i];
+  }
   __syncthreads();
-  before_count = sh.before_count, before_mass = sh.before_mass;
-  const int found = sh.found;
+  before_count = __builtin_amdgcn_readfirstlane(sh.before_count), before_mass = uniform(sh.before_mass);
+  const int found = __builtin_amdgcn_readfirstlane(sh.found);
   __syncthreads();
   return found;
 }
@@ -206,18 +236,21 @@ __device__ __forceinline__ void fill(Histogram& h, const Src& src, const Scale& 
 
 // total weight of a histogram, on every thread
 __device__ __forceinline__ u64 total_mass(Shared& sh, const Histogram& h) {
-  const u64 v = wave_sum(h.mass[2 * threadIdx.x] + h.mass[2 * threadIdx.x + 1]);
+  u64 v = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) v += h.mass[kPer * threadIdx.x + i];
+  v = wave_sum(v);
   if (threadIdx.x % kWave == 0) sh.wave_a[threadIdx.x / kWave] = v;
   __syncthreads();
   u64 s = 0;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) s += sh.wave_a[i];
   __syncthreads();
-  return s;
+  return uniform(s);
 }
 
 __device__ __forceinline__ u64 share(double p, u64 total) {        // the weight that top-p asks for
-  const u64 need = static_cast<u64>(ceil(p * static_cast<double>(total)));
+  const u64 need = uniform(static_cast<u64>(ceil(p * static_cast<double>(total))));
   return min(max(need, u64{1}), total);
 }
 
@@ -227,7 +260,7 @@ __device__ __forceinline__ u64 share(double p, u64 total) {        // the weight
 template <typename Src>
 __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, bool by_mass, bool masses,
                                           u64 need, unsigned count, u64& mass) {
-  const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   u64 lo = 0, hi = ~u64{0};
   auto members = [&](auto f) {
     src([&](float l, int i) {
@@ -259,19 +292,21 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
       __syncthreads();
       lo = sh.wave_a[0], hi = sh.wave_b[0];
       for (int i = 1; i < kWaves; ++i) lo = min(lo, sh.wave_a[i]), hi = max(hi, sh.wave_b[i]);
+      lo = uniform(lo), hi = uniform(hi);
     }
     // all places differ: a turn leaves at most 1 / 1024 of the range, and single places at last
     const int shift = max(0, 53 - __clzll(static_cast<long long>(hi - lo)));
-    clear(sh.sub);
+    if (t == 0) sh.divided = true;
+    clear(sh.hist);
     members([&](u64 at, double d) {
       const int digit = static_cast<int>((hi - at) >> shift);
-      if (!by_mass) atomicAdd(&sh.sub.count[digit], 1u);
-      if (masses) atomicAdd(&sh.sub.mass[digit], whole(sc.weight(d)));
+      if (!by_mass) atomicAdd(&sh.hist.count[digit], 1u);
+      if (masses) atomicAdd(&sh.hist.mass[digit], whole(sc.weight(d)));
     });
     __syncthreads();
     unsigned bc;
     u64 bm;
-    const int digit = min(find_bin(sh, sh.sub, by_mass, need - (by_mass ? mass : count), bc, bm), kBins - 1);
+    const int digit = min(find_bin(sh, sh.hist, by_mass, need - (by_mass ? mass : count), bc, bm), kBins - 1);
     count += bc, mass += bm;
     hi -= static_cast<u64>(digit) << shift;
     lo = max(lo, hi - ((u64{1} << shift) - 1));
@@ -293,8 +328,8 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
     if (before < need && need <= before + own) sh.limit = at, sh.limit_mass = mass + mb + w;
   }
   __syncthreads();
-  mass = sh.limit_mass;
-  const u64 limit = sh.limit;
+  mass = uniform(sh.limit_mass);
+  const u64 limit = uniform(sh.limit);
   __syncthreads();
   return limit;
 }
@@ -345,30 +380,38 @@ __device__ __forceinline__ float group_max(float v, float* red) {
   __syncthreads();
   v = red[0];
   for (int i = 1; i < static_cast<int>(blockDim.x) / kWave; ++i) v = fmaxf(v, red[i]);
-  return v;
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
 }
 
-// ---- one workgroup a row, NV vectors of scores a thread ---------------------------------------------------------------------
-template <typename T, int NV>
+// ---- one workgroup a row, the row in LDS ------------------------------------------------------------------------------------
+// In registers the compiler keeps what one pass derives from a score for the next, for every score, and spills (69 us instead of
+// 43 for 512 rows of 10677).  A pass over the row in LDS is ~1 us; what bounds a row is its chain of about fifteen barriers.
+template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g) {
   __shared__ Shared sh;
-  __shared__ Histogram hist;
   __shared__ float red[kWaves];
-  constexpr int V = 16 / sizeof(T);
-  const int row = blockIdx.x, t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  __shared__ u64 part[kLevels * kWaves];
+  extern __shared__ __attribute__((aligned(16))) char lds_row[];
+  constexpr int V = 4, LEVEL = kThreads * V;
+  static_assert(kLevels * kWaves <= kWave, "one lane a part");
+  const int row = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
+  pack<T, V>* mine = reinterpret_cast<pack<T, V>*>(lds_row) + t;        // level i of a thread: mine[i * kThreads]
   const Row r = row_settings(g, row);
-  float x[NV][V];
+  const int levels = (g.n + LEVEL - 1) / LEVEL;
   float top = -__builtin_inff();
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int base = (i * kThreads + t) * V, n = g.n - base;
-    load_vec<T, V>(x[i], l + base, n);
+  for (int i = 0; i < levels; ++i) {
+    const int base = i * LEVEL + t * V, n = g.n - base;
+    float x[V];
+    load_vec<T, V>(x, l + base, n);
+    pack<T, V> a;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (j >= n) x[i][j] = -__builtin_inff();
-      top = fmaxf(top, x[i][j]);
+      if (j >= n) x[j] = -__builtin_inff();
+      a.v[j] = from_f32<T>(x[j]);
+      top = fmaxf(top, x[j]);
     }
+    mine[i * kThreads] = a;
   }
   top = group_max(top, red);
   if (top == -__builtin_inff()) {                        // nothing to draw from (also N = 0)
@@ -377,54 +420,58 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
   }
   const Scale sc = scale_of(top, r, g.bits);
   auto src = [&](auto f) {
+#pragma unroll 1
+    for (int i = 0; i < levels; ++i) {
+      const int base = i * LEVEL + t * V;
+      if (base >= g.n) break;
+      const pack<T, V> a = mine[i * kThreads];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) f(x[i][j], (i * kThreads + t) * V + j);
+      for (int j = 0; j < V; ++j) f(to_f32(a.v[j]), base + j);
+    }
   };
-  u64 limit = 0;
-  if (r.k > 0 || r.by_p) {
-    fill(hist, src, sc, r.k > 0, r.by_p);
+  u64 limit = 0, total_weight = 0;                       // of the row, then of the top-k items
+  bool filled = false;
+#pragma unroll 1
+  for (int by_mass = 0; by_mass < 2; ++by_mass) {        // top-k, then top-p
+    if (by_mass ? !r.by_p : r.k == 0) continue;
+    if (!filled) {
+      if (t == 0) sh.divided = false;
+      fill(sh.hist, src, sc, r.k > 0, r.by_p);
+      if (total_weight == 0 && r.by_p) total_weight = total_mass(sh, sh.hist);
+    }
+    const u64 need = by_mass ? share(r.p, total_weight) : static_cast<u64>(r.k);
     unsigned count;
-    u64 mass, total = r.by_p ? total_mass(sh, hist) : 0;
-    if (r.k > 0) {
-      const int b = find_bin(sh, hist, false, static_cast<u64>(r.k), count, mass);
-      if (b < kBins) {
-        limit = find_limit(sh, src, sc, b, b, false, r.by_p, static_cast<u64>(r.k), count, mass);
-        total = mass;
-      }
+    u64 mass;
+    const int b = find_bin(sh, sh.hist, by_mass, need, count, mass);
+    if (b < kBins) {
+      limit = max(limit, find_limit(sh, src, sc, b, b, by_mass, r.by_p, need, count, mass));
+      total_weight = mass;
     }
-    if (r.by_p) {
-      const u64 need = share(r.p, total);
-      const int b = find_bin(sh, hist, true, need, count, mass);
-      if (b < kBins) limit = max(limit, find_limit(sh, src, sc, b, b, true, true, need, count, mass));
-    }
+    filled = !sh.divided;
   }
   // kept weight by index: level i of wave w comes after level i of wave w - 1, and after every wave's level i - 1
-  __shared__ u64 part[NV * kWaves];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  auto weights = [&](int i, u64 (&w)[V]) {
+    const int base = i * LEVEL + t * V;
+    const pack<T, V> a = mine[i * kThreads];
     u64 sum = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum += kept(x[i][j], (i * kThreads + t) * V + j, sc, limit, r.m);
-    sum = wave_sum(sum);
+    for (int j = 0; j < V; ++j) w[j] = kept(to_f32(a.v[j]), base + j, sc, limit, r.m), sum += w[j];
+    return sum;
+  };
+  u64 w[V];
+#pragma unroll 1
+  for (int i = 0; i < levels; ++i) {
+    const u64 sum = wave_sum(weights(i, w));
     if (lane == 0) part[i * kWaves + wave] = sum;
   }
   __syncthreads();
-  static_assert(NV * kWaves <= kWave, "one lane a part");
-  const u64 mine = lane < NV * kWaves ? part[lane] : 0, total = wave_sum(mine), goal = goal_of(g.u[row], total);
-  u64 before = wave_before(mine);
-  const int owner = __ffsll(static_cast<unsigned long long>(__ballot(before <= goal && goal < before + mine))) - 1;
+  const u64 own = lane < levels * kWaves ? part[lane] : 0, total = wave_sum(own), goal = goal_of(g.u[row], total);
+  u64 before = wave_before(own);
+  const int owner = __ffsll(static_cast<unsigned long long>(__ballot(before <= goal && goal < before + own))) - 1;
   if (owner % kWaves != wave) return;
-  before = __shfl(before, owner);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (owner / kWaves == i) {
-      u64 w[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) w[j] = kept(x[i][j], (i * kThreads + t) * V + j, sc, limit, r.m);
-      draw<V>(g, row, (i * kThreads + t) * V, w, goal, total, before);
-    }
+  before = from_lane(before, owner);
+  weights(owner / kWaves, w);
+  draw<V>(g, row, owner / kWaves * LEVEL + t * V, w, goal, total, before);
 }
 
 // ---- long rows ----------------------------------------------------------------------------------------------------------------
@@ -486,26 +533,31 @@ __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const Sample
 
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs g) {
   __shared__ Shared sh;
-  __shared__ Histogram hist;
+  Histogram& hist = sh.hist;
   const int row = blockIdx.x, t = threadIdx.x;
   const Row r = row_settings(g, row);
   RowState s{0, 0, 0, 0, kBins, kBins, kBins};
   if (r.k > 0 || r.by_p) {
-    const long long at = static_cast<long long>(row) * g.pieces * kBins + 2 * t;      // this thread's two bins
-    u64 m0 = 0, m1 = 0;
-    unsigned c0 = 0, c1 = 0;
-#pragma unroll 8
-    for (int z = 0; z < g.pieces; ++z) {
+    for (int j = 2 * t; j < kBins; j += 2 * kThreads) {
+      const long long at = static_cast<long long>(row) * g.pieces * kBins + j;
+      u64 m0 = 0, m1 = 0;
+      unsigned c0 = 0, c1 = 0;
       if (r.by_p) {
-        const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(g.mass + at + static_cast<long long>(z) * kBins);
-        m0 += m.x, m1 += m.y;
+#pragma unroll 8
+        for (int z = 0; z < g.pieces; ++z) {
+          const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(g.mass + at + static_cast<long long>(z) * kBins);
+          m0 += m.x, m1 += m.y;
+        }
       }
       if (r.k > 0) {
-        const uint2 c = *reinterpret_cast<const uint2*>(g.count + at + static_cast<long long>(z) * kBins);
-        c0 += c.x, c1 += c.y;
+#pragma unroll 8
+        for (int z = 0; z < g.pieces; ++z) {
+          const uint2 c = *reinterpret_cast<const uint2*>(g.count + at + static_cast<long long>(z) * kBins);
+          c0 += c.x, c1 += c.y;
+        }
       }
+      hist.mass[j] = m0, hist.mass[j + 1] = m1, hist.count[j] = c0, hist.count[j + 1] = c1;
     }
-    hist.mass[2 * t] = m0, hist.mass[2 * t + 1] = m1, hist.count[2 * t] = c0, hist.count[2 * t + 1] = c1;
     __syncthreads();
     u64 most = 0, least = 0;                             // the weight of the top-k items lies between them
     if (r.by_p) least = most = s.total = total_mass(sh, hist);
@@ -531,7 +583,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) {
   __shared__ unsigned listed;
   constexpr int V = 16 / sizeof(T), U = 4;
-  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   const Row r = row_settings(g, row);
   const Scale sc = scale_of(row_top(g, row), r, g.bits);
@@ -577,7 +629,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   __shared__ Shared sh;
   __shared__ u64 chunk[kChunks], lds_list[kListed];
   constexpr int V = 16 / sizeof(T);
-  const int row = blockIdx.x, t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+  const int row = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   const Row r = row_settings(g, row);
   const float top = row_top(g, row);
@@ -605,14 +657,14 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     }
     whole_list = whole_list && listed <= kListed;
     auto limits = [&](auto src) {
-      u64 mass = s.k_mass, total = s.total;
-      if (s.k_bin < kBins) {
-        limit = find_limit(sh, src, sc, s.k_bin, s.k_bin, false, r.by_p, static_cast<u64>(r.k), s.k_count, mass);
+      u64 total = s.total;
+#pragma unroll 1
+      for (int by_mass = 0; by_mass < 2; ++by_mass) {    // top-k, then top-p
+        if ((by_mass ? s.p_lo : s.k_bin) == kBins) continue;
+        u64 mass = by_mass ? s.p_mass : s.k_mass;
+        limit = max(limit, find_limit(sh, src, sc, by_mass ? s.p_lo : s.k_bin, by_mass ? s.p_hi : s.k_bin, by_mass, r.by_p,
+                                      by_mass ? share(r.p, total) : static_cast<u64>(r.k), s.k_count, mass));
         total = mass;
-      }
-      if (s.p_lo < kBins) {
-        mass = s.p_mass;
-        limit = max(limit, find_limit(sh, src, sc, s.p_lo, s.p_hi, true, true, share(r.p, total), 0, mass));
       }
     };
     if (whole_list) {
@@ -658,8 +710,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   if (before <= goal && goal < before + mine)
     for (at = c0; before + chunk[at] <= goal; ++at) before += chunk[at];
   const int owner = __ffsll(static_cast<unsigned long long>(__ballot(at >= 0))) - 1;
-  at = __shfl(at, owner);
-  before = __shfl(before, owner);
+  at = __builtin_amdgcn_readlane(at, owner);
+  before = from_lane(before, owner);
   const int end = min(g.n, (at + 1) * g.span);
   for (int base0 = at * g.span; base0 < end; base0 += kWave * V) {
     const int base = base0 + lane * V;
@@ -672,8 +724,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   }
 }
 
-// items a workgroup holds in registers
-constexpr int kRowItems = 16384;
+// items of a row that one workgroup holds
+constexpr int kRowItems = kLevels * kThreads * 4;
 
 // long rows: the workspace, from `base` on (null: its size alone)
 inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* base) {
@@ -706,13 +758,10 @@ inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* ba
 template <typename T>
 void launch(const SampleArgs& g, bool limits, hipStream_t st) {
   const dim3 rows(static_cast<unsigned>(g.rows)), block(kThreads);
-  constexpr int V = 16 / sizeof(T);
-  if (g.n <= kThreads * V) {
-    hipLaunchKernelGGL((sample_row_kernel<T, 1>), rows, block, 0, st, g);
-  } else if (g.n <= 2 * kThreads * V) {
-    hipLaunchKernelGGL((sample_row_kernel<T, 2>), rows, block, 0, st, g);
-  } else if (g.n <= kRowItems) {
-    if constexpr (V == 4) hipLaunchKernelGGL((sample_row_kernel<T, 4>), rows, block, 0, st, g);
+  constexpr int LEVEL = kThreads * 4;
+  if (g.n <= kRowItems) {
+    const size_t lds = static_cast<size_t>((g.n + LEVEL - 1) / LEVEL) * LEVEL * sizeof(T);
+    hipLaunchKernelGGL(sample_row_kernel<T>, rows, block, lds, st, g);
   } else {
     const dim3 pieces(static_cast<unsigned>(g.rows) * g.pieces);
     hipLaunchKernelGGL(sample_top_kernel<T>, pieces, dim3(256), 0, st, g);
@@ -731,9 +780,10 @@ void launch(const SampleArgs& g, bool limits, hipStream_t st) {
 using namespace sg;
 
 SG_API size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n, int dtype) {
-  if (rows <= 0 || n <= kRowItems || n >= SG_SAMPLE_MAX_ITEMS || !valid_dtype(dtype)) return 0;
+  if (rows <= 0 || n >= SG_SAMPLE_MAX_ITEMS || !valid_dtype(dtype)) return 0;
+  const int size = dtype == SG_DTYPE_F32 ? 4 : 2;
   SampleArgs g{};
-  return lay_out(g, rows, n, dtype == SG_DTYPE_F32 ? 4 : 2, nullptr);
+  return n <= kRowItems ? 0 : lay_out(g, rows, n, size, nullptr);
 }
 
 SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld, int dtype, const float* u, int64_t rows,
@@ -748,8 +798,10 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
   if (ld < n) return fail(SG_ERR_INVALID, "sample_rows: rows overlap");
   if (!(temperature >= 0.0) || !(top_p >= 0.0) || !(min_p >= 0.0) || top_k < 0)
     return fail(SG_ERR_INVALID, "sample_rows: temperature, top_k, top_p and min_p must not be negative");
-  if (n > kRowItems && rows * kMaxPieces >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
-  if (workspace_bytes < sg_sample_rows_workspace_bytes(rows, n, dtype) || (n > kRowItems && !workspace))
+  const int size = dtype == SG_DTYPE_F32 ? 4 : 2;
+  const bool long_rows = n > kRowItems;
+  if (long_rows && rows * kMaxPieces >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
+  if (workspace_bytes < sg_sample_rows_workspace_bytes(rows, n, dtype) || (long_rows && !workspace))
     return fail(SG_ERR_WORKSPACE, "sample_rows workspace too small");
   int log_n = 0;
   while ((1ll << log_n) < n) ++log_n;
@@ -758,7 +810,7 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
   g.temperature = temperature_rows, g.top_k = top_k_rows, g.top_p = top_p_rows, g.min_p = min_p_rows;
   g.t0 = temperature, g.p0 = top_p, g.m0 = min_p, g.k0 = top_k;
   g.ld = ld, g.rows = static_cast<int>(rows), g.n = static_cast<int>(n), g.bits = std::min(51, 62 - log_n);
-  if (n > kRowItems) lay_out(g, rows, n, dtype == SG_DTYPE_F32 ? 4 : 2, static_cast<char*>(workspace));
+  if (long_rows) lay_out(g, rows, n, size, static_cast<char*>(workspace));
   // whether any row can have a limit: otherwise the histogram has no reader
   const bool limits = top_k_rows || top_p_rows || temperature_rows || min_p_rows || (top_k > 0 && top_k < n) || top_p < 1.0 ||
                       temperature == 0.0 || min_p > 1.0;
