@@ -165,30 +165,10 @@ struct Shared {
   int found;
 };
 
-// Sum of the lanes up to this one.  On the vector ALU (shifts inside rows of 16 lanes, then lanes 15 and 31 into the rows behind
-// them): a shuffle through LDS costs a hundred cycles a step.
-__device__ __forceinline__ u64 wave_upto(u64 v) {
-  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
-    constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
-    const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), C, R, 0xf, false);
-    const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), C, R, 0xf, false);
-    v += static_cast<u64>(hi) << 32 | lo;
-  };
-  using std::integral_constant;
-  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});      // row_shr:1, 2, 4, 8
-  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
-  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
-  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
-  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});      // row_bcast:15 into rows 1 and 3
-  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});      // row_bcast:31 into rows 2 and 3
-  return v;
+// sum of the lanes below this one
+__device__ __forceinline__ u64 wave_before(u64 v) {
+  return wave_scan(v, u64{0}, [](u64 a, u64 b) { return a + b; }) - v;
 }
-__device__ __forceinline__ u64 from_lane(u64 v, int lane) {
-  return static_cast<u64>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
-         static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
-}
-__device__ __forceinline__ u64 wave_sum(u64 v) { return from_lane(wave_upto(v), kWave - 1); }
-__device__ __forceinline__ u64 wave_before(u64 v) { return wave_upto(v) - v; }      // sum of the lanes below this one
 
 // The bin, counted from bin 0 on, in which the sum of counts reaches `need` (by_mass: the sum of weights), and the sums before
 // it; kBins if there is none.
@@ -375,7 +355,7 @@ __device__ __forceinline__ bool draw(const SampleArgs& g, int row, int base, con
 }
 
 __device__ __forceinline__ float group_max(float v, float* red) {
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+  v = wave_max(v);
   if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
   __syncthreads();
   v = red[0];
@@ -482,21 +462,28 @@ struct RowState {
   int k_bin, p_lo, p_hi;           // kBins: no such limit
 };
 
-// f(score, index) for the items [lo, hi) of a row, `threads` threads
+// f(score, index) for the items [lo, hi) of a row.  Whole vectors first, U loads under way at once
 template <typename T, typename F>
 __device__ __forceinline__ void each(const T* row, int lo, int hi, F f) {
-  constexpr int V = 16 / sizeof(T), U = 2;
-  const int step = blockDim.x * V;
-  for (int base = lo + threadIdx.x * V; base < hi; base += U * step) {
-    float x[U][V];
+  constexpr int V = 16 / sizeof(T), U = 4;
+  const int step = blockDim.x * V, end = lo + (hi - lo) / V * V;
+  int base = lo + threadIdx.x * V;
+  for (; base + (U - 1) * step < end; base += U * step) {
+    pack<T, V> a[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_vec<T, V>(x[u], row + base + u * step, hi - (base + u * step));
+    for (int u = 0; u < U; ++u) a[u] = load_pack<T, V>(row + base + u * step);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (base + u * step + j < hi) f(x[u][j], base + u * step + j);
+      for (int j = 0; j < V; ++j) f(to_f32(a[u].v[j]), base + u * step + j);
   }
+  for (; base < end; base += step) {
+    const pack<T, V> a = load_pack<T, V>(row + base);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f(to_f32(a.v[j]), base + j);
+  }
+  const int i = end + threadIdx.x;
+  if (i < hi) f(to_f32(row[i]), i);
 }
 
 template <typename T>
@@ -596,26 +583,34 @@ __global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) 
   for (int ch = c0 + wave; ch < c1; ch += 4) {
     u64 sum = 0;
     const int end = min(g.n, (ch + 1) * g.span);
-    for (int base = ch * g.span + lane * V; base < end; base += U * kWave * V) {
-      float x[U][V];
+    auto item = [&](float x, int i) {
+      const double d = sc.below(x);
+      if (!sc.live(d)) return;
+      const int b = sc.bin(d);
+      if (surely_kept(s, b)) {
+        const double w = sc.weight(d);
+        if (w >= r.m) sum += whole(w);
+      } else if (candidate(s, b)) {
+        const unsigned k = atomicAdd(&listed, 1u);
+        if (k < static_cast<unsigned>(g.room)) list[k] = place(x, i);
+      }
+    };
+    int base = ch * g.span + lane * V;
+    if ((ch + 1) * g.span <= g.n) {                      // a whole chunk: a multiple of U vectors a lane
+      for (; base < end; base += U * kWave * V) {
+        pack<T, V> a[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) load_vec<T, V>(x[u], l + base + u * kWave * V, end - (base + u * kWave * V));
+        for (int u = 0; u < U; ++u) a[u] = load_pack<T, V>(l + base + u * kWave * V);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int i = base + u * kWave * V + j;
-          const double d = sc.below(x[u][j]);
-          if (i >= end || !sc.live(d)) continue;
-          const int b = sc.bin(d);
-          if (surely_kept(s, b)) {
-            const double w = sc.weight(d);
-            if (w >= r.m) sum += whole(w);
-          } else if (candidate(s, b)) {
-            const unsigned k = atomicAdd(&listed, 1u);
-            if (k < static_cast<unsigned>(g.room)) list[k] = place(x[u][j], i);
-          }
-        }
+          for (int j = 0; j < V; ++j) item(to_f32(a[u].v[j]), base + u * kWave * V + j);
+      }
+    } else {
+      for (; base < end; base += kWave * V)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (base + j < end) item(to_f32(l[base + j]), base + j);
     }
     sum = wave_sum(sum);
     if (lane == 0) g.chunk[static_cast<long long>(row) * g.chunks + ch] = sum;
