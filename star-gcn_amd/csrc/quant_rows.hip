@@ -101,9 +101,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void quant_rows_kernel(const
     for (int i = 0; i < WPR; ++i) ss += red[0][i], top = fmax(top, red[1][i]);
   }
   if (!live) return;
-  const double rstd = g.norm ? 1.0 / sqrt(ss / g.dim + g.eps) : 1.0 + ss * 0.0;
+  const double rstd = !g.norm ? 1.0 : top == 0.0 ? 0.0 : 1.0 / sqrt(ss / g.dim + g.eps);      // zeros stay zeros, whatever eps
   float scale = static_cast<float>(top * rstd / 127.0);
-  const bool none = !(scale <= 3.402823466e38f) || !(rstd <= 1.7976931348623157e308);      // NaN and infinities
+  const bool none = ss != ss || !(scale <= 3.402823466e38f);        // NaN and infinities
   if (none) scale = __builtin_nanf("");
   if (t == 0) g.scale[row] = scale;
   const double s = scale, inv = (none || scale == 0.f) ? 0.0 : 1.0 / s;
@@ -172,6 +172,8 @@ SG_API int sg_quant_rows_i8_hip(int8_t* codes, float* scale, void* sum, const vo
   if (rows == 0) return SG_OK;
   if (!codes || !scale || !x) return fail(SG_ERR_INVALID, "quant_rows: null pointer argument");
   if (ldx < dim || (residual && ldr < dim)) return fail(SG_ERR_INVALID, "quant_rows: rows overlap");
+  if (sum && rows > 1 && ((sum == x && ldx != dim) || (sum == residual && ldr != dim)))
+    return fail(SG_ERR_INVALID, "quant_rows: a sum in place needs rows without gaps");
   QuantArgs g{codes, scale, sum, x, residual, weight, ldx, ldr, rows, static_cast<int>(dim), norm, weight_f32, eps};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == SG_DTYPE_F32) dispatch<float>(g, st);

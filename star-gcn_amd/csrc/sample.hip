@@ -35,7 +35,7 @@ constexpr int kPer = kBins / kThreads;
 constexpr int kFew = 512;          // candidates that are ranked against each other
 constexpr int kChunks = 4096;      // partial weights by index of a long row
 constexpr int kListed = 8192;      // candidates of a long row's limits
-constexpr int kMaxPieces = 32;
+constexpr int kMaxPieces = 32, kMaxParts = 128;
 constexpr int kLevels = 4096 / kThreads;      // groups of four that a thread holds of a short row
 
 typedef unsigned long long u64;
@@ -53,13 +53,14 @@ struct SampleArgs {
   long long ld, k0;
   int rows, n, bits;               // bits: s above
   // long rows: pieces of `piece` items, chunks of `span`; workspace
-  int pieces, piece, span, chunks, room;
-  float* tops;                     // (rows, pieces)
+  // and, for the passes that leave little behind, parts of `part` items
+  int pieces, piece, parts, part, span, chunks, room;
+  float* tops;                     // (rows, parts)
   u64* mass;                       // (rows, pieces, kBins)
   unsigned* count;
   struct RowState* state;          // (rows)
-  unsigned* listed;                // (rows, pieces): candidates of the piece, which may be more than `room`
-  u64* list;                       // (rows, pieces, room): their places in the order
+  unsigned* listed;                // (rows, parts): candidates of the part, which may be more than `room`
+  u64* list;                       // (rows, parts, room): their places in the order
   u64* chunk;                      // (rows, chunks): weight of what is surely kept
 };
 
@@ -489,17 +490,17 @@ __device__ __forceinline__ void each(const T* row, int lo, int hi, F f) {
 template <typename T>
 __global__ __launch_bounds__(256) void sample_top_kernel(const SampleArgs g) {
   __shared__ float red[4];
-  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, lo = z * g.piece;
+  const int row = blockIdx.x / g.parts, z = blockIdx.x % g.parts, lo = z * g.part;
   float top = -__builtin_inff();
-  each(static_cast<const T*>(g.l) + row * g.ld, lo, min(g.n, lo + g.piece), [&](float x, int) { top = fmaxf(top, x); });
+  each(static_cast<const T*>(g.l) + row * g.ld, lo, min(g.n, lo + g.part), [&](float x, int) { top = fmaxf(top, x); });
   top = group_max(top, red);
   if (threadIdx.x == 0) g.tops[blockIdx.x] = top;
 }
 
 __device__ __forceinline__ float row_top(const SampleArgs& g, int row) {
-  float top = g.tops[row * g.pieces];
-  for (int i = 1; i < g.pieces; ++i) top = fmaxf(top, g.tops[row * g.pieces + i]);
-  return top;
+  float top = -__builtin_inff();
+  for (int i = threadIdx.x % kWave; i < g.parts; i += kWave) top = fmaxf(top, g.tops[row * g.parts + i]);
+  return wave_max(top);
 }
 
 template <typename T>
@@ -525,26 +526,27 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
   const Row r = row_settings(g, row);
   RowState s{0, 0, 0, 0, kBins, kBins, kBins};
   if (r.k > 0 || r.by_p) {
-    for (int j = 2 * t; j < kBins; j += 2 * kThreads) {
-      const long long at = static_cast<long long>(row) * g.pieces * kBins + j;
-      u64 m0 = 0, m1 = 0;
-      unsigned c0 = 0, c1 = 0;
-      if (r.by_p) {
+    static_assert(kPer == 4, "16 bytes of counts a thread");
+    const long long at = static_cast<long long>(row) * g.pieces * kBins + kPer * t;      // this thread's bins
+    u64 m[kPer] = {};
+    unsigned c[kPer] = {};
+    if (r.by_p) {
 #pragma unroll 8
-        for (int z = 0; z < g.pieces; ++z) {
-          const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(g.mass + at + static_cast<long long>(z) * kBins);
-          m0 += m.x, m1 += m.y;
-        }
+      for (int z = 0; z < g.pieces; ++z) {
+        const ulonglong2* p = reinterpret_cast<const ulonglong2*>(g.mass + at + static_cast<long long>(z) * kBins);
+        const ulonglong2 a = p[0], b = p[1];
+        m[0] += a.x, m[1] += a.y, m[2] += b.x, m[3] += b.y;
       }
-      if (r.k > 0) {
-#pragma unroll 8
-        for (int z = 0; z < g.pieces; ++z) {
-          const uint2 c = *reinterpret_cast<const uint2*>(g.count + at + static_cast<long long>(z) * kBins);
-          c0 += c.x, c1 += c.y;
-        }
-      }
-      hist.mass[j] = m0, hist.mass[j + 1] = m1, hist.count[j] = c0, hist.count[j + 1] = c1;
     }
+    if (r.k > 0) {
+#pragma unroll 8
+      for (int z = 0; z < g.pieces; ++z) {
+        const uint4 a = *reinterpret_cast<const uint4*>(g.count + at + static_cast<long long>(z) * kBins);
+        c[0] += a.x, c[1] += a.y, c[2] += a.z, c[3] += a.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) hist.mass[kPer * t + i] = m[i], hist.count[kPer * t + i] = c[i];
     __syncthreads();
     u64 most = 0, least = 0;                             // the weight of the top-k items lies between them
     if (r.by_p) least = most = s.total = total_mass(sh, hist);
@@ -565,12 +567,13 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
 __device__ __forceinline__ bool surely_kept(const RowState& s, int bin) { return bin < s.k_bin && bin < s.p_lo; }
 __device__ __forceinline__ bool candidate(const RowState& s, int bin) { return bin == s.k_bin || (bin >= s.p_lo && bin <= s.p_hi); }
 
-// one wave a chunk of the piece
+// one wave a chunk of the part
 template <typename T>
-__global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) {
+__global__ __launch_bounds__(256) void sample_parts_kernel(const SampleArgs g) {
   __shared__ unsigned listed;
   constexpr int V = 16 / sizeof(T), U = 4;
-  const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int row = blockIdx.x / g.parts, z = blockIdx.x % g.parts;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   const Row r = row_settings(g, row);
   const Scale sc = scale_of(row_top(g, row), r, g.bits);
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(256) void sample_pieces_kernel(const SampleArgs g) 
   u64* list = g.list + static_cast<long long>(blockIdx.x) * g.room;
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
-  const int c0 = z * (g.piece / g.span), c1 = min(g.chunks, c0 + g.piece / g.span);
+  const int c0 = z * (g.part / g.span), c1 = min(g.chunks, c0 + g.part / g.span);
   for (int ch = c0 + wave; ch < c1; ch += 4) {
     u64 sum = 0;
     const int end = min(g.n, (ch + 1) * g.span);
@@ -638,16 +641,16 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   for (int i = t; i < g.chunks; i += kThreads) chunk[i] = g.chunk[static_cast<long long>(row) * g.chunks + i];
   u64 limit = 0;
   if (s.k_bin < kBins || s.p_lo < kBins) {
-    // the pieces' lists, one behind the other in LDS if they fit
+    // the parts' lists, one behind the other in LDS if they fit
     int listed = 0;
     bool whole_list = true;
-    for (int z = 0; z < g.pieces; ++z) {
-      const unsigned n = g.listed[row * g.pieces + z];
+    for (int z = 0; z < g.parts; ++z) {
+      const unsigned n = g.listed[row * g.parts + z];
       whole_list = whole_list && n <= static_cast<unsigned>(g.room);
       if (!whole_list) break;
       if (z % kWaves == wave)
         for (int i = lane; i < static_cast<int>(n) && listed + i < kListed; i += kWave)
-          lds_list[listed + i] = g.list[(static_cast<long long>(row) * g.pieces + z) * g.room + i];
+          lds_list[listed + i] = g.list[(static_cast<long long>(row) * g.parts + z) * g.room + i];
       listed += static_cast<int>(n);
     }
     whole_list = whole_list && listed <= kListed;
@@ -728,24 +731,28 @@ inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* ba
   g.span = static_cast<int>(4 * kWave * vec);            // four vectors a lane
   while ((n + g.span - 1) / g.span > kChunks) g.span *= 2;
   g.chunks = static_cast<int>((n + g.span - 1) / g.span);
-  // enough pieces for four workgroups a compute unit, of at least 8192 items
-  const int64_t want = std::min<int64_t>({kMaxPieces, std::max<int64_t>(1, 1024 / rows), std::max<int64_t>(1, n / 8192)});
-  const int64_t per = (g.chunks + want - 1) / want;
-  g.piece = static_cast<int>(std::min<int64_t>(per * g.span, int64_t{1} << 30));
-  g.pieces = static_cast<int>((g.chunks + per - 1) / per);
-  g.room = std::min(kListed, g.piece / 4);
+  // enough for four workgroups a compute unit, of at least 8192 items (a piece leaves a histogram to be read: 32 a row at most)
+  auto cut = [&](int64_t most, int& count, int& length) {
+    const int64_t want = std::min<int64_t>({most, std::max<int64_t>(1, 1024 / rows), std::max<int64_t>(1, n / 8192)});
+    const int64_t per = (g.chunks + want - 1) / want;    // chunks
+    length = static_cast<int>(std::min<int64_t>(per * g.span, int64_t{1} << 30));
+    count = static_cast<int>((g.chunks + per - 1) / per);
+  };
+  cut(kMaxPieces, g.pieces, g.piece);
+  cut(kMaxParts, g.parts, g.part);
+  g.room = std::min(kListed, g.part / 4);
   size_t at = 0;
   auto take = [&](auto*& p, size_t count) {
     p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
     at += (count * sizeof(*p) + 255) & ~size_t{255};
   };
-  const size_t all = static_cast<size_t>(rows) * g.pieces;
-  take(g.tops, all);
-  take(g.mass, all * kBins);
-  take(g.count, all * kBins);
+  const size_t pieces = static_cast<size_t>(rows) * g.pieces, parts = static_cast<size_t>(rows) * g.parts;
+  take(g.tops, parts);
+  take(g.mass, pieces * kBins);
+  take(g.count, pieces * kBins);
   take(g.state, rows);
-  take(g.listed, all);
-  take(g.list, all * g.room);
+  take(g.listed, parts);
+  take(g.list, parts * g.room);
   take(g.chunk, static_cast<size_t>(rows) * g.chunks);
   return at;
 }
@@ -758,13 +765,13 @@ void launch(const SampleArgs& g, bool limits, hipStream_t st) {
     const size_t lds = static_cast<size_t>((g.n + LEVEL - 1) / LEVEL) * LEVEL * sizeof(T);
     hipLaunchKernelGGL(sample_row_kernel<T>, rows, block, lds, st, g);
   } else {
-    const dim3 pieces(static_cast<unsigned>(g.rows) * g.pieces);
-    hipLaunchKernelGGL(sample_top_kernel<T>, pieces, dim3(256), 0, st, g);
+    const dim3 pieces(static_cast<unsigned>(g.rows) * g.pieces), parts(static_cast<unsigned>(g.rows) * g.parts);
+    hipLaunchKernelGGL(sample_top_kernel<T>, parts, dim3(256), 0, st, g);
     if (limits) {
       hipLaunchKernelGGL(sample_histogram_kernel<T>, pieces, block, 0, st, g);
       hipLaunchKernelGGL(sample_bins_kernel, rows, block, 0, st, g);
     }
-    hipLaunchKernelGGL(sample_pieces_kernel<T>, pieces, dim3(256), 0, st, g);
+    hipLaunchKernelGGL(sample_parts_kernel<T>, parts, dim3(256), 0, st, g);
     hipLaunchKernelGGL(sample_draw_kernel<T>, rows, block, 0, st, g);
   }
 }
@@ -795,7 +802,7 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
     return fail(SG_ERR_INVALID, "sample_rows: temperature, top_k, top_p and min_p must not be negative");
   const int size = dtype == SG_DTYPE_F32 ? 4 : 2;
   const bool long_rows = n > kRowItems;
-  if (long_rows && rows * kMaxPieces >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
+  if (long_rows && rows * kMaxParts >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
   if (workspace_bytes < sg_sample_rows_workspace_bytes(rows, n, dtype) || (long_rows && !workspace))
     return fail(SG_ERR_WORKSPACE, "sample_rows workspace too small");
   int log_n = 0;

@@ -173,7 +173,7 @@ def l2_loss(pred, target, scale):
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, student, teacher, ids, scale, temperature):
-        ids = L.i32c(ids)
+        ids = ops._item_ids(ids)
         loss, stats, p = ops.distill_fwd(student, teacher, ids, scale, temperature)
         ctx.scale, ctx.temperature = scale, temperature
         ctx.save_for_backward(student, ids, stats, p)

@@ -544,28 +544,40 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if not torch.is_tensor(v):
             return v, None
         L.require_current_gpu(v)
-        if v.dtype != dtype and v.is_floating_point() != dtype.is_floating_point:
+        if v.is_floating_point() != dtype.is_floating_point or v.dtype == torch.bool:
             raise L.StarGCNError("sample_rows: %s cannot be of %s" % (name, v.dtype))
-        v = v if v.dtype == dtype else v.to(dtype)
-        return 0, _vector(v.view(1) if v.dim() == 0 and rows == 1 else v, rows, dtype, "sample_rows " + name)
+        if v.dtype != dtype:
+            v = v.to(dtype) if dtype.is_floating_point else v.clamp(max=0x7fffffff).to(dtype)
+        return 0, _vector(v.expand(rows) if v.dim() == 0 else v, rows, dtype, "sample_rows " + name)
 
     (t, tr), (p, pr), (m, mr) = (setting(v, torch.float32, name) for v, name in
                                  ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
     k, kr = setting(top_k, torch.int32, "top_k")
+    if kr is None and int(k) != k:
+        raise L.StarGCNError("sample_rows: top_k has to be a whole number, got %r" % (k,))
     ids = torch.empty((rows,), dtype=torch.int32, device=logits.device)
     prob = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     lib = L.lib()
     wsn = lib.sg_sample_rows_workspace_bytes(rows, n, dt)
     ws = L.scratch(wsn, logits.device)
-    L.check(lib.sg_sample_rows_hip(L.ptr(ids), L.ptr(prob), L.ptr(logits), ld, dt, L.ptr(u), rows, n, float(t), int(k), float(p),
+    L.check(lib.sg_sample_rows_hip(L.ptr(ids), L.ptr(prob), L.ptr(logits), ld, dt, L.ptr(u), rows, n, float(t), min(int(k), n), float(p),
                                    float(m), L.ptr(tr), L.ptr(kr), L.ptr(pr), L.ptr(mr), L.ptr(ws), wsn, L.stream_ptr()),
             "sg_sample_rows_hip")
     return ids, prob
 
 
+def _item_ids(ids):
+    """ids as int32; what int32 cannot hold is no item either way."""
+    if ids.is_floating_point() or ids.dtype == torch.bool:
+        raise L.StarGCNError("distill_loss: ids have to be whole numbers, got %s" % ids.dtype)
+    return L.i32c(ids.clamp(-1, 0x7fffffff) if ids.dtype == torch.int64 else ids)
+
+
 def _distill_shapes(student, teacher, ids):
     L.require_current_gpu(student, teacher, ids)
     _dtype_id(student, "distill_loss")
+    if not teacher.is_floating_point():
+        raise L.StarGCNError("distill_loss: the teacher's scores have to be floating point, got %s" % teacher.dtype)
     if teacher.dim() != 2 or teacher.shape != ids.shape or student.dim() != 2 or teacher.shape[0] != student.shape[0]:
         raise L.StarGCNError("distill_loss: student (rows, items), teacher scores and ids (rows, k) expected, got %s, %s and %s" %
                              (tuple(student.shape), tuple(teacher.shape), tuple(ids.shape)))
@@ -575,7 +587,7 @@ def distill_fwd(student, teacher, ids, scale, temperature=1.0):
     """-> (loss, stats, p) of sg_distill_hip; functional.distill_loss is the differentiable form."""
     _distill_shapes(student, teacher, ids)
     student, ld = _rows(student, "distill_loss")
-    teacher, ids = L.f32c(teacher), L.i32c(ids)
+    teacher, ids = L.f32c(teacher), _item_ids(ids)
     (rows, n), k = student.shape, teacher.shape[1]
     loss = torch.empty((), dtype=torch.float32, device=student.device)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=student.device)
@@ -593,7 +605,7 @@ def distill_bwd(grad_loss, student, stats, p, ids, scale, temperature=1.0):
     """The gradient of distill_fwd's loss for the student's scores (contiguous, the student's type)."""
     L.require_current_gpu(grad_loss, student, stats, p, ids)
     student, ld = _rows(student, "distill_loss")
-    ids = L.i32c(ids)
+    ids = _item_ids(ids)
     rows, n = student.shape
     grad = torch.empty((rows, n), dtype=student.dtype, device=student.device)
     L.check(L.lib().sg_distill_bwd_hip(L.ptr(grad), L.ptr(student), ld, L.DTYPE[student.dtype], L.ptr(stats), L.ptr(p), L.ptr(ids),

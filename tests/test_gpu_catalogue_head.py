@@ -84,6 +84,23 @@ def test_codes_of_ties_zeros_and_extreme_rows():
     assert ops.quantize_rows(x.to(DEV))[1][7].item() == 0.0
 
 
+def test_zeros_have_scale_zero_whatever_eps():
+    x = torch.zeros(3, 100, device=DEV)
+    x[1] = 2.0
+    codes, scale, _ = ops.rms_norm_i8(x, eps=0.0)
+    assert scale.tolist() == [0.0, float(np.float32(1.0 / 127)), 0.0] and (codes[1] == 127).all() and (codes[::2] == 0).all()
+
+
+def test_the_sum_may_replace_the_residual():
+    x, r = (torch.randn(70, 300, generator=gen(k)).to(DEV) for k in (1, 2))
+    want = ops.rms_norm_i8(x, None, residual=r)
+    codes, scale = torch.empty(70, 300, dtype=torch.int8, device=DEV), torch.empty(70, device=DEV)
+    args = lambda ldr: (L.ptr(codes), L.ptr(scale), L.ptr(r), L.ptr(x), 300, L.ptr(r), ldr, None, 0, 70, 300, 0, 1, 1e-6, L.stream_ptr())      # noqa: E731
+    assert L.lib().sg_quant_rows_i8_hip(*args(301)) == -1      # rows with gaps cannot be replaced by a sum without
+    L.check(L.lib().sg_quant_rows_i8_hip(*args(300)))
+    assert torch.equal(r, want[2]) and torch.equal(codes, want[0]) and torch.equal(scale, want[1])
+
+
 @pytest.mark.parametrize("norm", [False, True])
 def test_a_row_that_is_not_finite_has_no_codes_and_harms_no_other(norm):
     x = torch.randn(9, 333, generator=gen(1))
@@ -111,7 +128,7 @@ def check_product(a, sa, b, sb, bias, act, out):
     tol = 2.0 ** -24 * (2 * t.abs() + v.abs()) * 1.01 + (8 * 2.0 ** -24 * ref.abs() + 2.0 ** -24 if act in ("sigmoid", "tanh") else 2.0 ** -24 * ref.abs())
     fi = torch.finfo(out.dtype)
     tol = tol + (fi.eps / 2 * ref.abs() + fi.smallest_normal * fi.eps if out.dtype != torch.float32 else 0)
-    err = (out.double().cpu() - ref).abs()
+    err = (out.double().to(ref.device) - ref).abs()
     assert (err <= tol * 1.01 + 1e-45).all(), float((err - tol).max())
 
 
@@ -148,6 +165,31 @@ def test_product_of_long_rows_and_few(M, N, K):
 def test_product_types_and_activations(dtype, act):
     for M, N, K in ((3, 50, 64), (130, 200, 250), (260, 520, 1024)):
         product_case(M, N, K, dtype=dtype, act=act)
+
+
+@pytest.mark.parametrize("M,N", [(2000, 2050), (2049, 4099), (4000, 4100)])      # 128 x 128, 128 x 256 and 256 x 256 tiles
+@pytest.mark.parametrize("K", [64, 200, 250, 256, 512, 528, 600, 640, 1040])
+def test_product_of_large_matrices(M, N, K):
+    g = torch.Generator(device=DEV).manual_seed(K)
+    a, b = (torch.randint(-128, 128, (n, K), generator=g, device=DEV, dtype=torch.int16).to(torch.int8) for n in (M, N))
+    sa, sb, bias = (torch.rand(n, generator=g, device=DEV) + 0.1 for n in (M, N, N))
+    for dtype, act in ((torch.float32, None), (torch.bfloat16, None), (torch.float16, "tanh")):
+        s = 1.0 if dtype != torch.float16 else 1e-5
+        out = ops.gemm_i8(a, sa * s, b, sb, bias=bias, act=act, slope=0.2, out_dtype=dtype)
+        check_product(a, sa * s, b, sb, bias, act, out)
+    wide = torch.zeros(M, N + 9, device=DEV)
+    ops.gemm_i8(a, sa, b, sb, out=wide[:, 4:N + 4])
+    check_product(a, sa, b, sb, None, None, wide[:, 4:N + 4])
+    assert (wide[:, :4] == 0).all() and (wide[:, N + 4:] == 0).all()
+
+
+def test_product_larger_than_the_infinity_cache():
+    g = torch.Generator(device=DEV).manual_seed(1)
+    a, b = (torch.randint(-128, 128, (n, 96), generator=g, device=DEV, dtype=torch.int16).to(torch.int8) for n in (8200, 8208))
+    sa, sb = (torch.rand(n, generator=g, device=DEV) for n in (8200, 8208))
+    out = ops.gemm_i8(a, sa, b, sb)
+    for rows in (slice(0, 300), slice(4000, 4300), slice(7950, 8200)):
+        check_product(a[rows], sa[rows], b, sb, None, None, out[rows])
 
 
 def test_product_at_the_integers_limit():
@@ -289,6 +331,17 @@ def test_draw_with_settings_of_each_row():
     check_draw(l, torch.rand(32, generator=g), top_k=torch.arange(32))
 
 
+def test_draw_with_settings_on_the_device():
+    l, u = torch.randn(5, 400, generator=gen(1)), torch.rand(5, generator=gen(2))
+    want = ops.sample_rows(l.to(DEV), u.to(DEV), temperature=0.5, top_k=30, top_p=0.75)
+    one = lambda v, t: torch.tensor(v, dtype=t, device=DEV)      # noqa: E731
+    got = ops.sample_rows(l.to(DEV), u.to(DEV), temperature=one(0.5, torch.float64), top_k=one(30, torch.int64), top_p=one(0.75, torch.float16))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    many = ops.sample_rows(l.to(DEV), u.to(DEV), top_k=torch.full((5,), (1 << 32) + 1, device=DEV))
+    assert torch.equal(many[0], ops.sample_rows(l.to(DEV), u.to(DEV))[0])
+    assert torch.equal(ops.sample_rows(l.to(DEV), u.to(DEV), top_k=1 << 40)[0], many[0])
+
+
 def test_draw_from_slices_and_transposed_scores():
     big = (2 * torch.randn(20, 5003, generator=gen(9))).to(DEV)
     u = torch.rand(20, generator=gen(10))
@@ -421,6 +474,9 @@ def test_distill_of_padding_masks_and_items_named_twice():
     s[8, :100] = -INF
     ids[8] = torch.arange(200, 212)
     check_distill(s, t, ids)
+    far = ids.long()
+    far[0, 5], far[7, 2] = (1 << 32) + 7, -(1 << 40)       # no item, in 64 bits either
+    check_distill(s, t, far)
     x = s.to(DEV).requires_grad_(True)
     loss = SF.distill_loss(x, t.to(DEV), ids.to(DEV), 1.0)
     loss.backward()
@@ -617,7 +673,9 @@ def test_refusals_on_tensors():
            lambda: ops.gemm_i8(torch.zeros(1, 131072, dtype=torch.int8, device=DEV), s[:1], torch.zeros(1, 131072, dtype=torch.int8, device=DEV), s[:1]),
            lambda: ops.sample_rows(x, s[:3]), lambda: ops.sample_rows(x, s.double()), lambda: ops.sample_rows(x.double(), s),
            lambda: ops.sample_rows(x, s, temperature=-1.0), lambda: ops.sample_rows(x, s, top_k=-1), lambda: ops.sample_rows(x, s, top_p=math.nan),
-           lambda: ops.sample_rows(x, s, min_p=-0.5), lambda: ops.sample_rows(x, s, temperature=s[:2]), lambda: ops.sample_rows(x, s, top_k=torch.ones(4)),
+           lambda: ops.sample_rows(x, s, min_p=-0.5), lambda: ops.sample_rows(x, s, temperature=s[:2]), lambda: ops.sample_rows(x, s, top_k=torch.ones(4, device=DEV)),
+           lambda: ops.sample_rows(x, s, top_k=2.5), lambda: ops.sample_rows(x, s, top_p=s.cpu()), lambda: ops.sample_rows(x, s, top_p=s > 0),
+           lambda: SF.distill_loss(x, x, x, 1.0), lambda: SF.distill_loss(x, c, c.int(), 1.0),
            lambda: SF.distill_loss(x, x[:3], c[:3].int(), 1.0), lambda: SF.distill_loss(x, x, c[:, :4].int(), 1.0),
            lambda: SF.distill_loss(x.double(), x, c.int(), 1.0), lambda: SF.distill_loss(x, x, c.int(), 1.0, temperature=0.0),
            lambda: SF.distill_loss(x, torch.zeros(4, 1025, device=DEV), torch.zeros(4, 1025, dtype=torch.int32, device=DEV), 1.0),
