@@ -63,18 +63,23 @@ __device__ __forceinline__ void finish(const Args& g, T* c, int sum, float sa, f
   *c = from_f32<T>(act_fn(fmaf(static_cast<float>(sum) * sa, sb, bias), g.act, g.slope));
 }
 
-// 16 codes of a row from k on, zeros past K; any alignment
+// 16 codes of a row from k on, zeros past K; any alignment.  Where they end past K the row's last 16 are loaded and moved down, so
+// that no load hangs on a condition.
 __device__ __forceinline__ i32x4 load_codes(const int8_t* row, int k, int K) {
-  i32x4 v = {0, 0, 0, 0};
-  if (k + 16 <= K) {
-    v = *reinterpret_cast<const vec16_any*>(row + k);
-  } else if (k < K) {
-    int8_t b[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) b[j] = k + j < K ? row[k + j] : static_cast<int8_t>(0);
-    __builtin_memcpy(&v, b, 16);
+  if (K >= 16) {
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    const int at = min(k, K - 16), gone = (k - at) * 8;      // bits to move down
+    const u64x2 v = __builtin_bit_cast(u64x2, static_cast<vec16>(*reinterpret_cast<const vec16_any*>(row + at)));
+    const unsigned long long far = v[1] >> (gone & 63), near = (v[0] >> (gone & 63)) | (gone & 63 ? v[1] << (64 - (gone & 63)) : 0);
+    u64x2 r;
+    r[0] = gone < 64 ? near : gone < 128 ? far : 0;
+    r[1] = gone < 64 ? far : 0;
+    return __builtin_bit_cast(i32x4, r);
   }
-  return v;
+  int8_t b[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) b[j] = k + j < K ? row[k + j] : static_cast<int8_t>(0);
+  return __builtin_bit_cast(i32x4, b);
 }
 
 template <int N>
@@ -218,9 +223,15 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
   if (full < steps) {
     i32x4 v[PIECES];
     auto load = [&](int s) {
+      if ((s + 1) * BK <= k1 - k0) {                               // a whole step: nothing to look at
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-        v[i] = load_codes((i < PA ? pa : pb) + (off[i] - (DMA ? chunk(i) : 0)), s * BK + chunk(i), k1 - k0);
+        for (int i = 0; i < PIECES; ++i)
+          v[i] = *reinterpret_cast<const vec16_any*>((i < PA ? pa : pb) + (off[i] - (DMA ? chunk(i) : 0)) + s * BK + chunk(i));
+      } else {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+          v[i] = load_codes((i < PA ? pa : pb) + (off[i] - (DMA ? chunk(i) : 0)), s * BK + chunk(i), k1 - k0);
+      }
     };
     load(full);
     for (int s = full; s < steps; ++s) {

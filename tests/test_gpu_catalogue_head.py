@@ -364,6 +364,15 @@ def test_draw_from_long_rows(rows, n):
         check_draw(l, u, **kw)
 
 
+@pytest.mark.parametrize("n", [8191, 12289, 16383, 16384])
+def test_draw_from_the_longest_rows_of_one_workgroup(n):
+    g = gen(n)
+    for dtype in DTYPES:
+        l = (2 * torch.randn(3, n, generator=g)).to(dtype)
+        for kw in (dict(), dict(top_k=900, top_p=0.9), dict(top_p=0.999)):
+            check_draw(l, torch.rand(3, generator=g), **kw)
+
+
 def test_draws_follow_the_kept_distribution():
     l = torch.tensor([0.0, 1.0, 2.0, -1.0, 1.5], device=DEV)
     n = 200000
