@@ -4,7 +4,7 @@ Layout
   csrc/            hand-written HIP kernels + the C ABI (include/stargcn.h) -> libstargcn_hip.so
   _lib.py          ctypes binding of that library (fails loudly if it is missing; no CPU fallback)
   contrib.py       the `F.contrib.seg_*` operator surface of the reference on torch CUDA tensors
-  ops.py           thin wrappers of the C-ABI entry points (gather, seg ops, GEMM, fused aggregator, ...)
+  ops.py           thin wrappers of the C-ABI entry points (gather, seg ops, GEMM, fused aggregator, catalogue head, ...)
   functional.py    autograd glue: linear (Dense / FullyConnected on the matrix-core GEMM), multilink_aggregate, take_rows, ...
   plan.py          cached aggregation plans (fused multi-link CSR + transpose, source-range phases), host- or device-built
   device_graph.py  rating graph resident in HBM, plans built on the device; device_sampler.py / resident.py: per-batch work

@@ -221,17 +221,18 @@ __global__ __launch_bounds__(kThreads) void distill_join_kernel(const DistillArg
   finish_row(g, row, top, s, e);
 }
 
-__global__ __launch_bounds__(kThreads) void distill_sum_kernel(float* loss, const float* row_loss, int rows, double scale) {
-  __shared__ double red[kWaves];
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(float* loss, const float* row_loss, int rows, double scale) {
+  __shared__ double red[kSumThreads / kWave];
   double v = 0.0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < rows; i += kThreads) v += row_loss[i];
+#pragma unroll 8
+  for (int i = threadIdx.x; i < rows; i += kSumThreads) v += row_loss[i];
   v = wave_sum(v);
   if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
   __syncthreads();
   v = 0.0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) v += red[i];
+  for (int i = 0; i < kSumThreads / kWave; ++i) v += red[i];
   if (threadIdx.x == 0) *loss = static_cast<float>(scale * v);
 }
 
@@ -339,7 +340,7 @@ SG_API int sg_distill_hip(float* loss, float* stats, float* p, const void* stude
     else if (dtype == SG_DTYPE_F16) run(f16{});
     else run(bf16{});
   }
-  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kThreads), 0, st, loss, row_loss, static_cast<int>(rows),
+  hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kSumThreads), 0, st, loss, row_loss, static_cast<int>(rows),
                      static_cast<double>(scale) * temperature * temperature);
   return check_launch("distill");
 }

@@ -3,8 +3,8 @@
 //   C[m, n] = act( sa[m] * sb[n] * sum_k A[m, k] B[n, k] + bias[n] ),   A (M, K), B (N, K) row-major codes
 //
 // B holds one output channel a row (an item's row, a dense layer's weight as it is stored).  The sums are exact in 32-bit
-// integers (K < 2^17), so every kernel and every split of K gives the same bits; the epilogue rounds the sum to fp32, then
-// once for each of its two products, once for the bias and once to C's type.
+// integers (K < 2^17), so every kernel and every split of K gives the same bits; the epilogue rounds the sum to fp32, its product
+// with sa, the fused product with sb and bias, and the result to C's type.
 //
 // Tile kernel.  v_mfma_i32_32x32x32_i8: a lane feeds 16 consecutive k of one row of A and one of B, so both operands are used
 // exactly as they lie in memory.  A K step is 64 or 128 bytes of each of the tile's rows.  In LDS a row's 16-byte chunks sit at
@@ -15,10 +15,10 @@
 //   * Otherwise, and for the last step where K is no multiple of it: through registers, out-of-range k as zeros.
 // Rows past M or N are read as the last row; nothing is stored for them.
 //
-// What bounds it, measured on an MI355X.  8192 x 8192 x 4096, bf16 out: 281 us, 1.95 POP/s; the same with zero operands 181 us,
-// so it is the chip's power that sets the clock (1.7 GHz in the counters' runs), not the schedule; the matrix units are busy 55 %
-// of the cycles.  A K-short product (10000 x 10677 x 256 into fp32) is bound by its stores: 110 us, 3.9 TB/s against 6.6 TB/s of
-// a fill of the same buffer; odd row lengths cost it 10 %.  One row against 10677: the call's own latency.
+// What bounds it, measured on an MI355X.  8192 x 8192 x 4096 into bf16: 229 us, 2.4 POP/s, for quantised normal rows, 281 us for
+// uniformly random codes, 181 us for zeros: the chip's power sets the clock (1.7 GHz in the counters' runs), the matrix units are
+// busy 72 % of the cycles.  A K-short product (10000 x 10677 x 256 into fp32) is bound by its stores: 106 us, 4 TB/s against 6.6
+// TB/s of a fill of the same buffer; K = 250, through registers, takes 115.  One row against 10677: 4.5 us of a call of 12.
 #include "rows_shared.hpp"
 
 #include <algorithm>

@@ -8,7 +8,8 @@
 // A code is a decision at the border between two whole numbers, so everything up to it is held in 64 bits: the sum of
 // squares, y (an fp32 h times an fp32 w is exact in 64 bits) and the quotient.  The card's 64-bit vector rate makes that
 // cheap: ~10 operations an element against 7..13 bytes of memory traffic.  A row with an infinity or a NaN in it, or whose
-// scale overflows 32 bits, has no codes: scale NaN, codes 0, so that a product with it is NaN.  A row of zeros has scale 0.
+// scale overflows 32 bits, has no codes: scale NaN, codes 0, so that a product with it is NaN (0 behind relu, as the
+// library has it).  A row of zeros has scale 0.
 //
 // Memory bound: x and the residual are read once, codes and the sum written once; a row stays in the registers of its
 // threads between its reduction and its codes.  69878 x 256 fp32 with a residual: 43 us, 5.4 TB/s; 8192 x 4096 bf16: 50 us, 4.7

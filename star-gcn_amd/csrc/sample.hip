@@ -18,8 +18,8 @@
 // Rows of up to 16384 items: one workgroup a row, the row in LDS.  Longer rows are cut into pieces, five launches: maximum;
 // histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits and draw.
 // A list of more than 8192 candidates (many equal scores) is replaced by passes over the row.  64 rows of 1,000,000 fp32 scores,
-// top-p: 36 us for the maximum (6.9 TB/s), 88 for the histogram (bound by the 64-bit arithmetic and its LDS additions), 9, 62
-// and 9 for the rest.
+// top-p: 36 us for the maximum (6.9 TB/s), 79 for the histogram (bound by the 64-bit arithmetic: ~30 operations an item), 10, 54 and
+// 9 for the rest.
 #include "rows_shared.hpp"
 
 #include <algorithm>
@@ -114,20 +114,19 @@ __device__ __forceinline__ int index_at(u64 place) { return static_cast<int>(~st
 struct Scale {
   double top, c, last, bins;
   int bits;
-  bool endless;                    // max = +inf: only the items that equal it are live
 
-  __device__ __forceinline__ double below(float l) const {
-    const double d = (top - static_cast<double>(l)) * c;
-    return endless ? (static_cast<double>(l) == top ? 0.0 : 2.0 * last) : d;
-  }
+  // (max = +inf stands here as a number above every other score with an endless c: what equals it comes out as -inf, live, all
+  // else as +inf; live items' d is raised to 0 below)
+  __device__ __forceinline__ double below(float l) const { return (top - static_cast<double>(l)) * c; }
   __device__ __forceinline__ bool live(double d) const { return d < last; }
   // of a live item: 0 .. kBins - 2
   __device__ __forceinline__ int bin(double d) const {
-    return static_cast<int>(static_cast<unsigned>(__double_as_longlong(fma(d, bins, 6755399441055744.0))));
+    return static_cast<int>(static_cast<unsigned>(__double_as_longlong(fma(fmax(d, 0.0), bins, 6755399441055744.0))));
   }
   // of a live item: 2^(bits - d), to be rounded to a whole number.  2^f for |f| <= 1/2 by 1 + f times a polynomial that
   // interpolates (2^f - 1) / f at Chebyshev's points: 4e-14, and exact at f = 0
   __device__ __forceinline__ double weight(double d) const {
+    d = fmax(d, 0.0);
     const double t = d + 6755399441055744.0, f = (t - 6755399441055744.0) - d;
     double y = 1.0203121047189341e-07;
     y = fma(y, f, 1.3255224879317324e-06);
@@ -144,8 +143,9 @@ struct Scale {
   }
 };
 __device__ __forceinline__ Scale scale_of(float top, const Row& r, int bits) {
-  return Scale{uniform(static_cast<double>(top)), r.c, uniform(bits + 1.0), uniform((kBins - 2.0) / (bits + 1.0)), bits,
-               top == __builtin_inff()};
+  const bool endless = top == __builtin_inff();
+  return Scale{uniform(endless ? 1e39 : static_cast<double>(top)), uniform(endless ? 1e300 : r.c), uniform(bits + 1.0),
+               uniform((kBins - 2.0) / (bits + 1.0)), bits};
 }
 __device__ __forceinline__ u64 whole(double w) {                  // w < 2^52, to the nearest
   return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
@@ -161,9 +161,12 @@ struct Shared {
   bool divided;                    // a subdivision has replaced the row's
   u64 few_place[kFew], few_weight[kFew];
   u64 wave_a[kWaves], wave_b[kWaves];
-  u64 before_mass, limit, limit_mass;
-  unsigned before_count, few;
-  int found;
+  u64 limit, limit_mass;
+  unsigned few;
+  // of find_bin, two in turn: what one call leaves is read while the next one starts
+  u64 before_mass[2];
+  unsigned before_count[2];
+  int found[2];
 };
 
 // sum of the lanes below this one
@@ -171,40 +174,45 @@ __device__ __forceinline__ u64 wave_before(u64 v) {
   return wave_scan(v, u64{0}, [](u64 a, u64 b) { return a + b; }) - v;
 }
 
-// The bin, counted from bin 0 on, in which the sum of counts reaches `need` (by_mass: the sum of weights), and the sums before
-// it; kBins if there is none.
-__device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, bool by_mass, u64 need, unsigned& before_count, u64& before_mass) {
-  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
-  if (t == 0) sh.found = kBins, sh.before_count = 0, sh.before_mass = 0;
+// The bin, counted from bin 0 on, in which the sum of counts reaches need (by_mass: the sum of weights), need = need_of(total
+// weight), and the sums before it; kBins if there is none.  Two barriers; `turn` is the calls' own count.  Also starts an empty
+// list of candidates.
+template <typename Need>
+__device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, int& turn, bool by_mass, Need need_of, unsigned& before_count,
+                                        u64& before_mass) {
+  const int t = threadIdx.x, wave = t / kWave, lane = t % kWave, k = turn++ & 1;
+  if (t == 0) sh.found[k] = kBins, sh.before_count[k] = 0, sh.before_mass[k] = 0, sh.few = 0;
   u64 m[kPer], ms = 0;
   unsigned c[kPer], cs = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) m[i] = h.mass[kPer * t + i], c[i] = h.count[kPer * t + i], ms += m[i], cs += c[i];
-  u64 mb = wave_before(ms), cb = wave_before(cs);
+  u64 mb = wave_before(ms), cb = wave_before(u64{cs}), total = 0;
   if (lane == kWave - 1) sh.wave_a[wave] = mb + ms, sh.wave_b[wave] = cb + cs;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) mb += sh.wave_a[i], cb += sh.wave_b[i];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    total += sh.wave_a[i];
+    if (i < wave) mb += sh.wave_a[i], cb += sh.wave_b[i];
+  }
+  const u64 need = need_of(uniform(total));
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const u64 a = by_mass ? mb : cb, v = by_mass ? m[i] : c[i];
-    if (a < need && need <= a + v) sh.found = kPer * t + i, sh.before_count = static_cast<unsigned>(cb), sh.before_mass = mb;
+    if (a < need && need <= a + v) sh.found[k] = kPer * t + i, sh.before_count[k] = static_cast<unsigned>(cb), sh.before_mass[k] = mb;
     mb += m[i], cb += c[i];
   }
   __syncthreads();
-  before_count = __builtin_amdgcn_readfirstlane(sh.before_count), before_mass = uniform(sh.before_mass);
-  const int found = __builtin_amdgcn_readfirstlane(sh.found);
-  __syncthreads();
-  return found;
+  before_count = __builtin_amdgcn_readfirstlane(sh.before_count[k]), before_mass = uniform(sh.before_mass[k]);
+  return __builtin_amdgcn_readfirstlane(sh.found[k]);
 }
 
-__device__ __forceinline__ void clear(Histogram& h) {
+__device__ __forceinline__ void clear(Histogram& h) {              // a barrier has to follow
   for (int i = threadIdx.x; i < kBins; i += kThreads) h.mass[i] = 0, h.count[i] = 0;
-  __syncthreads();
 }
 
+// a cleared histogram
 template <typename Src>
 __device__ __forceinline__ void fill(Histogram& h, const Src& src, const Scale& sc, bool counts, bool masses) {
-  clear(h);
   src([&](float l, int) {
     const double d = sc.below(l);
     if (!sc.live(d)) return;
@@ -237,10 +245,10 @@ __device__ __forceinline__ u64 share(double p, u64 total) {        // the weight
 
 // The limit among the live items of `src` in bins lo_bin .. hi_bin, before which `count` items of weight `mass` stand in the
 // order: by count, the item with which the count reaches `need`; by mass, the item with which the weight does.  -> its place;
-// mass: with the item itself (by count only where `masses`).
+// mass: with the item itself (by count only where `masses`).  The list of candidates is empty.
 template <typename Src>
 __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, bool by_mass, bool masses,
-                                          u64 need, unsigned count, u64& mass) {
+                                          u64 need, unsigned count, u64& mass, int& turn) {
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   u64 lo = 0, hi = ~u64{0};
   auto members = [&](auto f) {
@@ -254,8 +262,6 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
     });
   };
   for (bool first = true;; first = false) {
-    if (t == 0) sh.few = 0, sh.limit = lo, sh.limit_mass = mass;
-    __syncthreads();
     members([&](u64 at, double d) {
       const unsigned k = atomicAdd(&sh.few, 1u);
       if (k < kFew) sh.few_place[k] = at, sh.few_weight[k] = masses ? whole(sc.weight(d)) : 0;
@@ -279,6 +285,7 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
     const int shift = max(0, 53 - __clzll(static_cast<long long>(hi - lo)));
     if (t == 0) sh.divided = true;
     clear(sh.hist);
+    __syncthreads();
     members([&](u64 at, double d) {
       const int digit = static_cast<int>((hi - at) >> shift);
       if (!by_mass) atomicAdd(&sh.hist.count[digit], 1u);
@@ -287,7 +294,8 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
     __syncthreads();
     unsigned bc;
     u64 bm;
-    const int digit = min(find_bin(sh, sh.hist, by_mass, need - (by_mass ? mass : count), bc, bm), kBins - 1);
+    const u64 rest = need - (by_mass ? mass : count);
+    const int digit = min(find_bin(sh, sh.hist, turn, by_mass, [&](u64) { return rest; }, bc, bm), kBins - 1);
     count += bc, mass += bm;
     hi -= static_cast<u64>(digit) << shift;
     lo = max(lo, hi - ((u64{1} << shift) - 1));
@@ -310,9 +318,7 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
   }
   __syncthreads();
   mass = uniform(sh.limit_mass);
-  const u64 limit = uniform(sh.limit);
-  __syncthreads();
-  return limit;
+  return uniform(sh.limit);
 }
 
 // the weight of an item if it is kept: its place is not below `limit`, the lower of the limits
@@ -366,7 +372,8 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 
 // ---- one workgroup a row, the row in LDS ------------------------------------------------------------------------------------
 // In registers the compiler keeps what one pass derives from a score for the next, for every score, and spills (69 us instead of
-// 43 for 512 rows of 10677).  A pass over the row in LDS is ~1 us; what bounds a row is its chain of about fifteen barriers.
+// 43 for 512 rows of 10677).  What bounds a row is 64-bit arithmetic on one compute unit, two passes of ~30 operations an item,
+// not its barriers (eleven instead of twenty: 16.4 -> 15.9 us for 10677 items).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g) {
   __shared__ Shared sh;
@@ -380,6 +387,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
   pack<T, V>* mine = reinterpret_cast<pack<T, V>*>(lds_row) + t;        // level i of a thread: mine[i * kThreads]
   const Row r = row_settings(g, row);
   const int levels = (g.n + LEVEL - 1) / LEVEL;
+  clear(sh.hist);
   float top = -__builtin_inff();
   for (int i = 0; i < levels; ++i) {
     const int base = i * LEVEL + t * V, n = g.n - base;
@@ -410,25 +418,28 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
       for (int j = 0; j < V; ++j) f(to_f32(a.v[j]), base + j);
     }
   };
-  u64 limit = 0, total_weight = 0;                       // of the row, then of the top-k items
-  bool filled = false;
+  u64 limit = 0, total = 0;                              // weight of the top-k items
+  int turn = 0;
+  bool again = false;
 #pragma unroll 1
   for (int by_mass = 0; by_mass < 2; ++by_mass) {        // top-k, then top-p
     if (by_mass ? !r.by_p : r.k == 0) continue;
-    if (!filled) {
+    if (again) clear(sh.hist), __syncthreads();
+    if (again || !turn) {
       if (t == 0) sh.divided = false;
       fill(sh.hist, src, sc, r.k > 0, r.by_p);
-      if (total_weight == 0 && r.by_p) total_weight = total_mass(sh, sh.hist);
     }
-    const u64 need = by_mass ? share(r.p, total_weight) : static_cast<u64>(r.k);
     unsigned count;
-    u64 mass;
-    const int b = find_bin(sh, sh.hist, by_mass, need, count, mass);
+    u64 mass, need = 0;
+    const int b = find_bin(sh, sh.hist, turn, by_mass, [&](u64 all) {
+      if (!by_mass || r.k == 0) total = all;
+      return need = by_mass ? share(r.p, total) : static_cast<u64>(r.k);
+    }, count, mass);
     if (b < kBins) {
-      limit = max(limit, find_limit(sh, src, sc, b, b, by_mass, r.by_p, need, count, mass));
-      total_weight = mass;
+      limit = max(limit, find_limit(sh, src, sc, b, b, by_mass, r.by_p, need, count, mass, turn));
+      total = mass;
     }
-    filled = !sh.divided;
+    again = sh.divided;
   }
   // kept weight by index: level i of wave w comes after level i of wave w - 1, and after every wave's level i - 1
   auto weights = [&](int i, u64 (&w)[V]) {
@@ -446,13 +457,13 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
     if (lane == 0) part[i * kWaves + wave] = sum;
   }
   __syncthreads();
-  const u64 own = lane < levels * kWaves ? part[lane] : 0, total = wave_sum(own), goal = goal_of(g.u[row], total);
+  const u64 own = lane < levels * kWaves ? part[lane] : 0, all = wave_sum(own), goal = goal_of(g.u[row], all);
   u64 before = wave_before(own);
   const int owner = __ffsll(static_cast<unsigned long long>(__ballot(before <= goal && goal < before + own))) - 1;
   if (owner % kWaves != wave) return;
   before = from_lane(before, owner);
   weights(owner / kWaves, w);
-  draw<V>(g, row, owner / kWaves * LEVEL + t * V, w, goal, total, before);
+  draw<V>(g, row, owner / kWaves * LEVEL + t * V, w, goal, all, before);
 }
 
 // ---- long rows ----------------------------------------------------------------------------------------------------------------
@@ -509,6 +520,8 @@ __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const Sample
   const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, lo = z * g.piece, hi = min(g.n, lo + g.piece);
   const Row r = row_settings(g, row);
   if (!(r.k > 0 || r.by_p)) return;
+  clear(hist);
+  __syncthreads();
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   fill(hist, [&](auto f) { each(l, lo, hi, f); }, scale_of(row_top(g, row), r, g.bits), r.k > 0, r.by_p);
   u64* mass = g.mass + static_cast<long long>(blockIdx.x) * kBins;
@@ -548,17 +561,18 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) hist.mass[kPer * t + i] = m[i], hist.count[kPer * t + i] = c[i];
     __syncthreads();
+    int turn = 0;
     u64 most = 0, least = 0;                             // the weight of the top-k items lies between them
     if (r.by_p) least = most = s.total = total_mass(sh, hist);
     if (r.k > 0) {
-      s.k_bin = find_bin(sh, hist, false, static_cast<u64>(r.k), s.k_count, s.k_mass);
+      s.k_bin = find_bin(sh, hist, turn, false, [&](u64) { return static_cast<u64>(r.k); }, s.k_count, s.k_mass);
       if (s.k_bin < kBins) least = s.k_mass, most = s.k_mass + hist.mass[s.k_bin];
     }
     if (r.by_p && s.total > 0) {                         // no total: a row of nothing but -inf and NaN
       unsigned c;
       u64 m;
-      s.p_hi = find_bin(sh, hist, true, share(r.p, most), c, m);
-      s.p_lo = least > 0 ? find_bin(sh, hist, true, share(r.p, least), c, s.p_mass) : 0;
+      s.p_hi = find_bin(sh, hist, turn, true, [&](u64) { return share(r.p, most); }, c, m);
+      s.p_lo = least > 0 ? find_bin(sh, hist, turn, true, [&](u64) { return share(r.p, least); }, c, s.p_mass) : 0;
     }
   }
   if (t == 0) g.state[row] = s;
@@ -655,13 +669,17 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     }
     whole_list = whole_list && listed <= kListed;
     auto limits = [&](auto src) {
+      int turn = 0;
       u64 total = s.total;
 #pragma unroll 1
       for (int by_mass = 0; by_mass < 2; ++by_mass) {    // top-k, then top-p
         if ((by_mass ? s.p_lo : s.k_bin) == kBins) continue;
         u64 mass = by_mass ? s.p_mass : s.k_mass;
+        __syncthreads();
+        if (t == 0) sh.few = 0;
+        __syncthreads();
         limit = max(limit, find_limit(sh, src, sc, by_mass ? s.p_lo : s.k_bin, by_mass ? s.p_hi : s.k_bin, by_mass, r.by_p,
-                                      by_mass ? share(r.p, total) : static_cast<u64>(r.k), s.k_count, mass));
+                                      by_mass ? share(r.p, total) : static_cast<u64>(r.k), s.k_count, mass, turn));
         total = mass;
       }
     };
