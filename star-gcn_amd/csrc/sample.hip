@@ -91,7 +91,7 @@ __device__ __forceinline__ Row row_settings(const SampleArgs& g, int row) {
   r.by_p = !(r.p >= 1.0);
   if (!(t > 0.0) || !(r.p > 0.0) || !(m <= 1.0)) r.k = 1;      // nothing but the first item
   if (r.k == 1) r.by_p = false, m = 0.0;
-  r.c = uniform(t > 0.0 ? 1.4426950408889634074 / t : 1.0);
+  r.c = uniform(t > 0.0 ? fmin(1.4426950408889634074 / t, 1e300) : 1.0);      // finite: the top's own 0 times it is 0
   r.m = uniform(m > 0.0 ? ldexp(m, g.bits) : 0.0);
   return r;
 }
@@ -823,6 +823,7 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
   if (long_rows && rows * kMaxParts >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
   if (workspace_bytes < sg_sample_rows_workspace_bytes(rows, n, dtype) || (long_rows && !workspace))
     return fail(SG_ERR_WORKSPACE, "sample_rows workspace too small");
+  if (long_rows && !aligned(workspace, 16)) return fail(SG_ERR_WORKSPACE, "sample_rows workspace has to be 16-byte aligned");
   int log_n = 0;
   while ((1ll << log_n) < n) ++log_n;
   SampleArgs g{};

@@ -331,6 +331,24 @@ def test_draw_with_settings_of_each_row():
     check_draw(l, torch.rand(32, generator=g), top_k=torch.arange(32))
 
 
+@pytest.mark.parametrize("n", [300, 40000])
+def test_draw_at_extreme_temperatures(n):
+    l = torch.randn(4, n, generator=gen(n))
+    l[1, 5] = INF
+    l[2] *= 1e38
+    l[3] *= 1e-38
+    u = torch.tensor([0.2, 0.4, 0.6, 0.8])
+    for T in (5e-324, 1e-320, 1e-300, 1e-45, 1e30, 1e300):
+        for kw in (dict(), dict(top_k=5), dict(top_p=0.9), dict(min_p=0.5, top_k=50, top_p=0.5)):
+            check_draw(l, u, temperature=T, **kw)
+    check_draw(l, u, temperature=torch.tensor([1e-45, 1e-40, 3e38, 1e-10]), top_p=0.9)
+    # every finite score alike, unless an infinite one (row 1's, and where 1e38 overflows row 2's) leaves the others nothing
+    ids, prob = ops.sample_rows(l.to(DEV), u.to(DEV), temperature=INF)
+    for i, row in enumerate(l):
+        alike = ((row == INF) if (row == INF).any() else row > -INF).nonzero().flatten()
+        assert ids[i].item() == alike[int(alike.numel() * float(u[i]))] and abs(prob[i].item() * alike.numel() - 1) < 1e-6
+
+
 def test_draw_with_settings_on_the_device():
     l, u = torch.randn(5, 400, generator=gen(1)), torch.rand(5, generator=gen(2))
     want = ops.sample_rows(l.to(DEV), u.to(DEV), temperature=0.5, top_k=30, top_p=0.75)
