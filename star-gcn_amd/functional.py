@@ -174,16 +174,16 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, student, teacher, ids, scale, temperature):
         ids = ops._item_ids(ids)
-        loss, stats, p = ops.distill_fwd(student, teacher, ids, scale, temperature)
+        loss, saved = ops.distill_fwd(student, teacher, ids, scale, temperature)
         ctx.scale, ctx.temperature = scale, temperature
-        ctx.save_for_backward(student, ids, stats, p)
+        ctx.save_for_backward(student, ids, saved)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        student, ids, stats, p = ctx.saved_tensors
-        return ops.distill_bwd(g, student, stats, p, ids, ctx.scale, ctx.temperature), None, None, None, None
+        student, ids, saved = ctx.saved_tensors
+        return ops.distill_bwd(g, student, saved, ids, ctx.scale, ctx.temperature), None, None, None, None
 
 
 def distill_loss(student, teacher, ids, scale, temperature=1.0):

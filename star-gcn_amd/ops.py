@@ -584,31 +584,32 @@ def _distill_shapes(student, teacher, ids):
 
 
 def distill_fwd(student, teacher, ids, scale, temperature=1.0):
-    """-> (loss, stats, p) of sg_distill_hip; functional.distill_loss is the differentiable form."""
+    """-> (loss, saved) of sg_distill_hip, saved = what distill_bwd needs: the rows' statistics (rows, 2) and shares (rows, k), then
+    the call's scratch memory, in one buffer.  functional.distill_loss is the differentiable form."""
     _distill_shapes(student, teacher, ids)
     student, ld = _rows(student, "distill_loss")
     teacher, ids = L.f32c(teacher), _item_ids(ids)
     (rows, n), k = student.shape, teacher.shape[1]
-    loss = torch.empty((), dtype=torch.float32, device=student.device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=student.device)
-    p = torch.empty((rows, k), dtype=torch.float32, device=student.device)
     lib = L.lib()
     wsn = lib.sg_distill_workspace_bytes(rows, n)
-    ws = L.scratch(wsn, student.device)
-    L.check(lib.sg_distill_hip(L.ptr(loss), L.ptr(stats), L.ptr(p), L.ptr(student), ld, L.DTYPE[student.dtype], L.ptr(teacher),
-                               L.ptr(ids), rows, n, k, float(temperature), float(scale), L.ptr(ws), wsn, L.stream_ptr()),
+    loss = torch.empty((), dtype=torch.float32, device=student.device)
+    saved = torch.empty(rows * (2 + k) + wsn // 4, dtype=torch.float32, device=student.device)
+    at = saved.data_ptr()
+    L.check(lib.sg_distill_hip(L.ptr(loss), at, at + 8 * rows, L.ptr(student), ld, L.DTYPE[student.dtype], L.ptr(teacher), L.ptr(ids),
+                               rows, n, k, float(temperature), float(scale), at + 4 * rows * (2 + k), wsn, L.stream_ptr()),
             "sg_distill_hip")
-    return loss, stats, p
+    return loss, saved
 
 
-def distill_bwd(grad_loss, student, stats, p, ids, scale, temperature=1.0):
+def distill_bwd(grad_loss, student, saved, ids, scale, temperature=1.0):
     """The gradient of distill_fwd's loss for the student's scores (contiguous, the student's type)."""
-    L.require_current_gpu(grad_loss, student, stats, p, ids)
+    L.require_current_gpu(grad_loss, student, saved, ids)
     student, ld = _rows(student, "distill_loss")
     ids = _item_ids(ids)
     rows, n = student.shape
     grad = torch.empty((rows, n), dtype=student.dtype, device=student.device)
-    L.check(L.lib().sg_distill_bwd_hip(L.ptr(grad), L.ptr(student), ld, L.DTYPE[student.dtype], L.ptr(stats), L.ptr(p), L.ptr(ids),
-                                       rows, n, p.shape[1], float(temperature), float(scale), L.ptr(L.f32c(grad_loss)),
-                                       L.stream_ptr()), "sg_distill_bwd_hip")
+    at = saved.data_ptr()
+    L.check(L.lib().sg_distill_bwd_hip(L.ptr(grad), L.ptr(student), ld, L.DTYPE[student.dtype], at, at + 8 * rows, L.ptr(ids), rows, n,
+                                       ids.shape[1], float(temperature), float(scale), L.ptr(L.f32c(grad_loss)), L.stream_ptr()),
+            "sg_distill_bwd_hip")
     return grad
