@@ -6,8 +6,8 @@
 // An entry whose id lies outside [0, N) or whose score is -inf is no entry.  A row without an entry, or whose student scores
 // are all -inf, has nothing to fit: it adds no loss and its gradient is zero.  An item that is named twice takes both shares.
 //
-// 10000 rows of 10677 bf16 scores: forward 55 us (3.9 TB/s; the chain of one row's entries shows), backward 90 us (4.7 TB/s, a
-// copy of that size reaches 5.3); 64 rows of 1,000,000 fp32: 45 and 89 us (5.7 TB/s).
+// 10000 rows of 10677 bf16 scores: forward 47 us (4.5 TB/s; the chain of one row's entries shows), backward 86 us (5.0 TB/s, a
+// copy of that size reaches 5.3); 64 rows of 1,000,000 fp32: 38 and 87 us (6.7 and 5.9 TB/s).
 //
 // Bound by memory: the forward reads the scores once (running maximum and sum, one exp an element), the backward reads them
 // again and writes the gradient; the K entries of a row are noise next to its N scores.  Long rows of small batches are split
@@ -35,6 +35,10 @@ struct DistillArgs {
   long long ld;
   int rows, n, k, splits, piece;
   float temperature, scale;
+  // Store the gradient past the caches: from 128 MB on scores and gradient together exceed the Infinity Cache, so a reader that
+  // starts at its beginning would not find it there, and writing it back delays whatever runs next.  64 x 1,000,000 fp32:
+  // backward 87 us instead of 91, the step 142 instead of 178; 10000 x 10677 bf16: 86 and 91, 145 and 164.
+  int past;
 };
 
 constexpr float kLowest = -3.402823466e38f, kLog2e = 1.442695040888963f;
@@ -255,12 +259,14 @@ __global__ __launch_bounds__(kThreads) void distill_bwd_kernel(const DistillArgs
   const float m = g.stats[2 * row], inv = g.stats[2 * row + 1], c = kLog2e / g.temperature;
   const bool none = inv == 0.f;
   const float f = g.scale * g.temperature * *g.gout, fq = f * inv;
+  const bool past = g.past && ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(sc)) & 15) == 0;
   auto slope = [&](T x) { return none ? 0.f : fq * exp2_fast((to_f32(x) - m) * c); };
   walk<4>(sc, lo, hi, [&](int i) { grad[i] = from_f32<T>(slope(sc[i])); },
            [&](pack<T, V> a, int at) {
 #pragma unroll
              for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(slope(a.v[j]));
-             store_pack<T, V>(grad + at, a);
+             if (past) __builtin_nontemporal_store(__builtin_bit_cast(vec16, a), reinterpret_cast<vec16*>(grad + at));
+             else store_pack<T, V>(grad + at, a);
            });
   if (none) return;
   // the teacher's items of this piece: the first entry that names an item writes it whole, the others' shares in entry order
@@ -329,7 +335,7 @@ SG_API int sg_distill_hip(float* loss, float* stats, float* p, const void* stude
   float* row_loss = static_cast<float*>(workspace);
   if (rows > 0) {
     DistillArgs g{student, teacher, ids, stats, p, row_loss + rows, row_loss, nullptr, nullptr, ld, static_cast<int>(rows),
-                  static_cast<int>(n), static_cast<int>(k), 0, 0, temperature, scale};
+                  static_cast<int>(n), static_cast<int>(k), 0, 0, temperature, scale, 0};
     split_rows(rows, n, &g.splits, &g.piece);
     auto run = [&](auto tag) {
       using T = decltype(tag);
@@ -352,7 +358,8 @@ SG_API int sg_distill_bwd_hip(void* grad, const void* student, int64_t ld, int d
   if (rows == 0) return SG_OK;
   if (!grad || !student || !stats || !grad_loss || (k > 0 && (!p || !ids))) return fail(SG_ERR_INVALID, "distill_bwd: null pointer argument");
   DistillArgs g{student, nullptr, ids, const_cast<float*>(stats), const_cast<float*>(p), nullptr, nullptr, grad, grad_loss, ld,
-                static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k), 0, 0, temperature, scale};
+                static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k), 0, 0, temperature, scale,
+                rows * n * (dtype == SG_DTYPE_F32 ? 4 : 2) >= (int64_t{128} << 20)};
   split_rows(rows, n, &g.splits, &g.piece);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(rows) * g.splits);
