@@ -469,6 +469,24 @@ def test_distill_of_long_rows(rows, n):
     check_distill(s, v, i.int(), T=1.0)
 
 
+@pytest.mark.parametrize("rows,n,dtype", [(34, 1000003, torch.float32), (900, 90001, torch.bfloat16), (520, 65536, torch.float32)])
+def test_distill_of_gradients_larger_than_the_cache(rows, n, dtype):
+    g = torch.Generator(device=DEV).manual_seed(n)
+    s = (2 * torch.randn(rows, n, generator=g, device=DEV)).to(dtype)
+    t = torch.randn(rows, 20, generator=g, device=DEV)
+    ids = torch.randint(0, n, (rows, 20), generator=g, device=DEV)
+    x = s.requires_grad_(True)
+    loss = SF.distill_loss(x, t, ids, 1.0 / rows, temperature=1.5)
+    grad, = torch.autograd.grad(loss, x)
+    f, fi = 1.5 / rows, torch.finfo(dtype)
+    for r in range(0, rows, 7):
+        q = torch.softmax(s[r].detach().double() / 1.5, 0)
+        p = torch.zeros_like(q).index_add_(0, ids[r], torch.softmax(t[r].double() / 1.5, 0))
+        want = f * (q - p)
+        # the bound of check_distill
+        assert ((grad[r].double() - want).abs() <= f * 7e-6 * (q + p) + fi.eps / 2 * want.abs() + fi.smallest_normal * fi.eps).all(), r
+
+
 def test_distill_gradient_against_differences():
     g = gen(2)
     s = torch.randn(1, 40, generator=g).to(DEV)
