@@ -18,8 +18,8 @@
 // Rows of up to 16384 items: one workgroup a row, the row in LDS.  Longer rows are cut into pieces, five launches: maximum;
 // histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits and draw.
 // A list of more than 8192 candidates (many equal scores) is replaced by passes over the row.  64 rows of 1,000,000 fp32 scores,
-// top-p: 36 us for the maximum (6.9 TB/s), 79 for the histogram (bound by the 64-bit arithmetic: ~30 operations an item), 10, 54 and
-// 9 for the rest.
+// top-p: 38 us for the maximum (6.7 TB/s), 61 for the histogram (bound by the 64-bit arithmetic: 24 operations an item), 10, 52 and
+// 12 for the rest.
 #include "rows_shared.hpp"
 
 #include <algorithm>
@@ -28,7 +28,7 @@
 namespace sg {
 namespace {
 
-// 512 threads and up to 128 registers: two workgroups a compute unit (512 rows of 10677: 31 us; of 1024 threads, one at a time: 43)
+// 512 threads and up to 128 registers: two workgroups a compute unit (512 rows of 10677: 28 us; of 1024 threads, one at a time: 43)
 constexpr int kThreads = 512, kWaves = kThreads / kWave;
 constexpr int kBins = 2048;        // of the histogram and of a subdivision
 constexpr int kPer = kBins / kThreads;
@@ -108,6 +108,22 @@ __device__ __forceinline__ float score_at(u64 place) {
 }
 __device__ __forceinline__ int index_at(u64 place) { return static_cast<int>(~static_cast<unsigned>(place)); }
 
+// (2^f - 1) / f for |f| <= 1/2: a polynomial that interpolates it at Chebyshev's points, to 4e-14 of 2^f.  Written out because the
+// compiler adds onto a copy of each coefficient, made for every item: 8 instructions of 34 (64 rows of 1,000,000: the histogram 61 us
+// instead of 79)
+__device__ __forceinline__ double exp2_slope(double f) {
+  double y;
+  asm("v_fma_f64 %0, %2, %1, %3\n\tv_fma_f64 %0, %0, %1, %4\n\tv_fma_f64 %0, %0, %1, %5\n\tv_fma_f64 %0, %0, %1, %6\n\t"
+      "v_fma_f64 %0, %0, %1, %7\n\tv_fma_f64 %0, %0, %1, %8\n\tv_fma_f64 %0, %0, %1, %9\n\tv_fma_f64 %0, %0, %1, %10"
+      : "=&v"(y)
+      : "v"(f), "v"(1.0203121047189341e-07), "s"(1.3255224879317324e-06), "s"(1.525268684635191e-05), "s"(0.0001540345585244999),
+        "s"(0.0013333558179042969), "s"(0.009618129159402565), "s"(0.055504108664760424), "s"(0.2402265069581299),
+        "s"(0.6931471805599453));
+  return y;
+}
+// max(d, 0) up to 2^-1022: a negative number's high half becomes 0
+__device__ __forceinline__ double raised(double d) { return __hiloint2double(max(__double2hiint(d), 0), __double2loint(d)); }
+
 // A row's scale: what turns a score into a bin of the histogram and into a weight.  d = (max - l) log2(e) / T; an item is live
 // if d < last: -inf, NaN and what lies so far below that its weight is 0 are not.  In the bit patterns: adding 1.5 * 2^52 to a
 // double rounds it to a whole number that stands in its low bits, for a quarter of a conversion's cost.
@@ -121,23 +137,13 @@ struct Scale {
   __device__ __forceinline__ bool live(double d) const { return d < last; }
   // of a live item: 0 .. kBins - 2
   __device__ __forceinline__ int bin(double d) const {
-    return static_cast<int>(static_cast<unsigned>(__double_as_longlong(fma(fmax(d, 0.0), bins, 6755399441055744.0))));
+    return static_cast<int>(static_cast<unsigned>(__double_as_longlong(fma(raised(d), bins, 6755399441055744.0))));
   }
-  // of a live item: 2^(bits - d), to be rounded to a whole number.  2^f for |f| <= 1/2 by 1 + f times a polynomial that
-  // interpolates (2^f - 1) / f at Chebyshev's points: 4e-14, and exact at f = 0
+  // of a live item: 2^(bits - d), to be rounded to a whole number.  exact at d = 0
   __device__ __forceinline__ double weight(double d) const {
-    d = fmax(d, 0.0);
+    d = raised(d);
     const double t = d + 6755399441055744.0, f = (t - 6755399441055744.0) - d;
-    double y = 1.0203121047189341e-07;
-    y = fma(y, f, 1.3255224879317324e-06);
-    y = fma(y, f, 1.525268684635191e-05);
-    y = fma(y, f, 0.0001540345585244999);
-    y = fma(y, f, 0.0013333558179042969);
-    y = fma(y, f, 0.009618129159402565);
-    y = fma(y, f, 0.055504108664760424);
-    y = fma(y, f, 0.2402265069581299);
-    y = fma(y, f, 0.6931471805599453);
-    y = fma(y, f, 1.0);
+    const double y = fma(exp2_slope(f), f, 1.0);
     const int n = static_cast<int>(static_cast<unsigned>(__double_as_longlong(t)));
     return __hiloint2double(__double2hiint(y) + (bits - n) * (1 << 20), __double2loint(y));
   }
@@ -372,7 +378,7 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 
 // ---- one workgroup a row, the row in LDS ------------------------------------------------------------------------------------
 // In registers the compiler keeps what one pass derives from a score for the next, for every score, and spills (69 us instead of
-// 43 for 512 rows of 10677).  What bounds a row is 64-bit arithmetic on one compute unit, two passes of ~30 operations an item,
+// 43 for 512 rows of 10677).  What bounds a row is 64-bit arithmetic on one compute unit, two passes of ~24 operations an item,
 // not its barriers (eleven instead of twenty: 16.4 -> 15.9 us for 10677 items).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g) {
