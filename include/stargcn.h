@@ -671,7 +671,8 @@ int sg_gemm_i8_hip(void* C, int64_t ldc, int dtype, const int8_t* A, int64_t lda
  * share top_p of the top-k items' weight (>= 1: all) and items with w_i >= min_p, but at least the first item.  ids[row] = the
  * first index at which the kept weight up to it exceeds u[row] times the kept weight, prob[row] = its share.  temperature 0,
  * top_p 0 or min_p > 1 leave the first item.  Scores of -inf and NaN are never drawn; a row of nothing else gets -1 and 0.
- * Settings are scalars, or one a row where the *_rows pointer is not NULL (values below 0 count as 0 there).  u in [0, 1). */
+ * Settings are scalars, or one a row where the *_rows pointer is not NULL (values below 0 count as 0 there).  u in [0, 1).
+ * Rows of more than 16384 items: fewer than 2^23 of them. */
 #define SG_SAMPLE_MAX_ITEMS (1 << 30)
 size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n, int dtype);
 int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld, int dtype, const float* u, int64_t rows, int64_t n,
@@ -685,7 +686,8 @@ int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld
  *   grad = grad_loss * scale * temperature * (q - p)
  * An id outside [0, n) or a teacher score of -inf is no entry; a row without an entry, or without a student score above -inf,
  * adds no loss and gets a zero gradient.  An item may be named more than once.  The forward leaves stats (rows, 2) and p
- * (rows, k) for the backward; grad (rows, n) is contiguous and of the student's type; grad_loss is one number on the device. */
+ * (rows, k) for the backward; grad (rows, n) is contiguous and of the student's type; grad_loss is one number on the device.
+ * Fewer than 2^24 rows and 2^30 items. */
 #define SG_DISTILL_MAX_K 1024
 size_t sg_distill_workspace_bytes(int64_t rows, int64_t n);
 int sg_distill_hip(float* loss, float* stats, float* p, const void* student, int64_t ld, int dtype, const float* teacher,

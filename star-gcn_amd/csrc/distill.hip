@@ -304,8 +304,8 @@ inline void split_rows(int64_t rows, int64_t n, int* splits, int* piece) {
 inline int check_args(const char* what, int dtype, int64_t ld, int64_t rows, int64_t n, int64_t k, float temperature) {
   if (!valid_dtype(dtype)) return fail(SG_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
   if (rows < 0 || n < 1 || k < 0) return fail(SG_ERR_INVALID, "%s: bad shape", what);
-  if (n >= (1ll << 30) || rows >= (1ll << 30) || k > SG_DISTILL_MAX_K)
-    return fail(SG_ERR_UNSUPPORTED, "%s: at most %d teacher entries a row, fewer than 2^30 rows and items", what, SG_DISTILL_MAX_K);
+  if (n >= (1ll << 30) || rows >= (1ll << 24) || k > SG_DISTILL_MAX_K)      // 2^32 threads a launch
+    return fail(SG_ERR_UNSUPPORTED, "%s: at most %d teacher entries a row, fewer than 2^24 rows and 2^30 items", what, SG_DISTILL_MAX_K);
   if (ld < n) return fail(SG_ERR_INVALID, "%s: rows overlap", what);
   if (!(temperature > 0.f) || !(temperature <= 3.402823466e38f)) return fail(SG_ERR_INVALID, "%s: temperature must be positive", what);
   return SG_OK;

@@ -408,7 +408,7 @@ SG_API int sg_gemm_i8_hip(void* C, int64_t ldc, int dtype, const int8_t* A, int6
   const int size = dtype == SG_DTYPE_F32 ? 4 : 2;
   // measured at 10000 x 10752 into fp32: 93 us past the caches, 99 through them
   g.nt = aligned(C, 16) && ldc * size % 16 == 0 && M * N * size > (256ll << 20);
-  if (static_cast<int64_t>(g.tiles_m) * g.tiles_n * s.splits >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "gemm_i8: too many tiles");
+  if (static_cast<int64_t>(g.tiles_m) * g.tiles_n * s.splits >= (1ll << 23)) return fail(SG_ERR_UNSUPPORTED, "gemm_i8: too many tiles");
   if (s.splits > 1 && (!workspace || workspace_bytes < sg_gemm_i8_workspace_bytes(M, N, K)))
     return fail(SG_ERR_WORKSPACE, "gemm_i8 workspace too small");
   const bool dma = aligned(A, 16) && aligned(B, 16) && lda % 16 == 0 && ldb % 16 == 0 && lda <= SG_GEMM_I8_MAX_K * 64 && ldb <= SG_GEMM_I8_MAX_K * 64;

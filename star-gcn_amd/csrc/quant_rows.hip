@@ -17,6 +17,8 @@
 #include "common.hpp"
 #include "rows_shared.hpp"
 
+#include <algorithm>
+
 namespace sg {
 namespace {
 
@@ -175,10 +177,15 @@ SG_API int sg_quant_rows_i8_hip(int8_t* codes, float* scale, void* sum, const vo
   if (ldx < dim || (residual && ldr < dim)) return fail(SG_ERR_INVALID, "quant_rows: rows overlap");
   if (sum && rows > 1 && ((sum == x && ldx != dim) || (sum == residual && ldr != dim)))
     return fail(SG_ERR_INVALID, "quant_rows: a sum in place needs rows without gaps");
-  QuantArgs g{codes, scale, sum, x, residual, weight, ldx, ldr, rows, static_cast<int>(dim), norm, weight_f32, eps};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == SG_DTYPE_F32) dispatch<float>(g, st);
-  else if (dtype == SG_DTYPE_F16) dispatch<f16>(g, st);
-  else dispatch<bf16>(g, st);
+  const int64_t size = dtype == SG_DTYPE_F32 ? 4 : 2, most = int64_t{1} << 21;      // a launch has to stay below 2^32 threads
+  for (int64_t r = 0; r < rows; r += most) {
+    auto of = [&](auto* p, int64_t ld) { return p ? reinterpret_cast<decltype(p)>(reinterpret_cast<uintptr_t>(p) + r * ld * size) : p; };
+    const QuantArgs g{codes + r * dim, scale + r, of(sum, dim), of(x, ldx), of(residual, ldr), weight, ldx, ldr, std::min(most, rows - r),
+                      static_cast<int>(dim), norm, weight_f32, eps};
+    if (dtype == SG_DTYPE_F32) dispatch<float>(g, st);
+    else if (dtype == SG_DTYPE_F16) dispatch<f16>(g, st);
+    else dispatch<bf16>(g, st);
+  }
   return check_launch("quant_rows");
 }

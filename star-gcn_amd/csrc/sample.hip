@@ -783,13 +783,23 @@ inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* ba
 
 template <typename T>
 void launch(const SampleArgs& g, bool limits, hipStream_t st) {
-  const dim3 rows(static_cast<unsigned>(g.rows)), block(kThreads);
+  const dim3 block(kThreads);
   constexpr int LEVEL = kThreads * 4;
   if (g.n <= kRowItems) {
     const size_t lds = static_cast<size_t>((g.n + LEVEL - 1) / LEVEL) * LEVEL * sizeof(T);
-    hipLaunchKernelGGL(sample_row_kernel<T>, rows, block, lds, st, g);
+    constexpr int most = 1 << 22;                        // a launch has to stay below 2^32 threads
+    for (long long r = 0; r < g.rows; r += most) {
+      SampleArgs a = g;
+      a.rows = static_cast<int>(std::min<long long>(most, g.rows - r));
+      a.ids += r, a.prob += r, a.u += r, a.l = static_cast<const T*>(g.l) + r * g.ld;
+      if (g.temperature) a.temperature += r;
+      if (g.top_k) a.top_k += r;
+      if (g.top_p) a.top_p += r;
+      if (g.min_p) a.min_p += r;
+      hipLaunchKernelGGL(sample_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), block, lds, st, a);
+    }
   } else {
-    const dim3 pieces(static_cast<unsigned>(g.rows) * g.pieces), parts(static_cast<unsigned>(g.rows) * g.parts);
+    const dim3 rows(static_cast<unsigned>(g.rows)), pieces(static_cast<unsigned>(g.rows) * g.pieces), parts(static_cast<unsigned>(g.rows) * g.parts);
     hipLaunchKernelGGL(sample_top_kernel<T>, parts, dim3(256), 0, st, g);
     if (limits) {
       hipLaunchKernelGGL(sample_histogram_kernel<T>, pieces, block, 0, st, g);
@@ -826,7 +836,7 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
     return fail(SG_ERR_INVALID, "sample_rows: temperature, top_k, top_p and min_p must not be negative");
   const int size = dtype == SG_DTYPE_F32 ? 4 : 2;
   const bool long_rows = n > kRowItems;
-  if (long_rows && rows * kMaxParts >= (1ll << 31)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
+  if (long_rows && rows >= (1ll << 23)) return fail(SG_ERR_UNSUPPORTED, "sample_rows: too many rows");
   if (workspace_bytes < sg_sample_rows_workspace_bytes(rows, n, dtype) || (long_rows && !workspace))
     return fail(SG_ERR_WORKSPACE, "sample_rows workspace too small");
   if (long_rows && !aligned(workspace, 16)) return fail(SG_ERR_WORKSPACE, "sample_rows workspace has to be 16-byte aligned");

@@ -50,7 +50,8 @@ NAN = float("nan")
     (lambda: distill(loss=None), -1), (lambda: distill(s=None), -1), (lambda: distill(t=None), -1), (lambda: distill(ids=None), -1),
     (lambda: distill(p=None), -1), (lambda: distill(stats=None), -1), (lambda: distill(ws=None), -5), (lambda: distill(wsn=1), -5),
     (lambda: distill_bwd(dtype=3), -1), (lambda: distill_bwd(grad=None), -1), (lambda: distill_bwd(g=None), -1), (lambda: distill_bwd(ld=7), -1),
-    (lambda: distill_bwd(k=1025), -2), (lambda: distill_bwd(temp=-1.0), -1), (lambda: distill_bwd(stats=None), -1), (lambda: distill_bwd(ids=None), -1),
+    (lambda: gemm(M=(1 << 30) - 1, N=1), -2), (lambda: sample(rows=1 << 23, n=20000, ld=20000), -2), (lambda: distill(rows=1 << 24), -2),
+    (lambda: distill_bwd(rows=1 << 24), -2), (lambda: distill_bwd(k=1025), -2), (lambda: distill_bwd(temp=-1.0), -1), (lambda: distill_bwd(stats=None), -1), (lambda: distill_bwd(ids=None), -1),
 ])
 def test_entry_points_refuse(call, code):
     assert call() == code

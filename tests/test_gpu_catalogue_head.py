@@ -38,6 +38,19 @@ def quant_reference(h, w, norm, eps):
     return codes.to(torch.int8), scale
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_codes_of_more_rows_than_one_launch_takes(dtype):
+    rows = (1 << 21) + 70
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(rows, 6, generator=g, device=DEV).to(dtype)[:, :5]
+    r = torch.randn(rows, 7, generator=g, device=DEV).to(dtype)[:, 2:]
+    w = torch.rand(5, generator=g, device=DEV).to(dtype)
+    codes, scale, h = ops.rms_norm_i8(x, w, residual=r)
+    assert torch.equal(h, x + r)
+    for cut in (slice(0, 64), slice((1 << 21) - 64, (1 << 21) + 64), slice(rows - 70, rows)):
+        check_codes((codes[cut], scale[cut]), quant_reference(h[cut].cpu(), w.cpu(), True, 1e-6))
+
+
 def check_codes(got, want):
     # both sides decide in 64 bits: a code differs only where the quotient lies within ~1e-13 of a tie, and the scale only
     # where the 64-bit value lies that near to the middle of two fp32 numbers; none does in these fixed inputs
@@ -389,6 +402,19 @@ def test_draw_from_the_longest_rows_of_one_workgroup(n):
         l = (2 * torch.randn(3, n, generator=g)).to(dtype)
         for kw in (dict(), dict(top_k=900, top_p=0.9), dict(top_p=0.999)):
             check_draw(l, torch.rand(3, generator=g), **kw)
+
+
+def test_draw_from_more_rows_than_one_launch_takes():
+    rows = (1 << 22) + 40
+    g = torch.Generator(device=DEV).manual_seed(6)
+    logits = torch.randn(rows, 4, generator=g, device=DEV)[:, :3]
+    u, t, p, m = (torch.rand(rows, generator=g, device=DEV) for _ in range(4))
+    k = torch.randint(0, 4, (rows,), generator=g, device=DEV)
+    ids, prob = ops.sample_rows(logits, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    for cut in (slice(0, 64), slice((1 << 22) - 64, (1 << 22) + 40)):
+        i, q = ops.sample_rows(logits[cut], u[cut], temperature=t[cut], top_k=k[cut], top_p=p[cut], min_p=m[cut])
+        assert torch.equal(ids[cut], i) and torch.equal(prob[cut], q)
+    assert ((ids >= 0) & (ids < 3)).all()
 
 
 def test_draws_follow_the_kept_distribution():
