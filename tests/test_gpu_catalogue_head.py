@@ -755,3 +755,21 @@ def test_refusals_on_tensors():
         with pytest.raises(L.StarGCNError):
             f()
             pytest.fail("call %d was not refused" % i)
+
+
+def test_distill_bwd_refuses_what_is_not_of_its_forward():
+    x, t = torch.randn(4, 50, device=DEV), torch.randn(4, 6, device=DEV)
+    ids = torch.randint(0, 50, (4, 6), device=DEV)
+    loss, saved = ops.distill_fwd(x, t, ids, 1.0)
+    one = torch.ones((), device=DEV)
+    grad = ops.distill_bwd(one, x, saved, ids, 1.0)
+    assert grad.shape == x.shape
+    bad = [(one, torch.randn(5, 50, device=DEV), saved, ids), (one, x, saved[:-1], ids), (one, x, saved.double(), ids), (one, x, saved[None], ids),
+           (one, x, torch.cat([saved, saved])[::2], ids), (one, x, saved, ids[:, :5]), (one, x, saved, ids[:3]), (one, x, saved, ids[0]),
+           (one, x, saved, torch.cat([ids, ids], 1)), (torch.ones(2, device=DEV), x, saved, ids), (one[None][:0], x, saved, ids),
+           (one, x.double(), saved, ids), (one, x[0], saved, ids), (one, x, saved.cpu(), ids), (one, x, saved, ids.float()),
+           (one, torch.randn(4, 20000, device=DEV), saved, ids)]
+    for i, (g, s, v, j) in enumerate(bad):
+        with pytest.raises(L.StarGCNError):
+            ops.distill_bwd(g, s, v, j, 1.0)
+            pytest.fail("call %d was not refused" % i)
