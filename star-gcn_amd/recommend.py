@@ -13,6 +13,25 @@ from . import _lib as L
 from . import ops
 
 
+def _mask_pairs(scores, rows, items):
+    """scores[rows[i], items[i]] = -inf; pairs outside the scores are passed over.  A minimum with +inf changes nothing, so this
+    needs neither a look at the indices on the host nor a list of the valid ones, and can be captured."""
+    L.require_current_gpu(scores, rows, items)
+    if rows.is_floating_point() or items.is_floating_point() or torch.bool in (rows.dtype, items.dtype):
+        raise L.StarGCNError("CatalogueHead: seen is a pair of index tensors, got %s and %s" % (rows.dtype, items.dtype))
+    try:
+        rows, items = torch.broadcast_tensors(rows, items)
+    except RuntimeError:
+        raise L.StarGCNError("CatalogueHead: seen's shapes %s and %s do not go together" % (tuple(rows.shape), tuple(items.shape)))
+    if not scores.numel() or not rows.numel():
+        return
+    m, n = scores.shape
+    rows, items = rows.reshape(-1).long(), items.reshape(-1).long()
+    inside = (rows >= 0) & (rows < m) & (items >= 0) & (items < n)
+    value = torch.full(inside.shape, float("inf"), dtype=scores.dtype, device=scores.device).masked_fill_(inside, -float("inf"))
+    scores.view(-1).scatter_reduce_(0, torch.where(inside, rows * n + items, torch.zeros_like(rows)), value, "amin")
+
+
 class CatalogueHead(object):
     """The item rows as 8-bit codes with one scale an item (a quarter of the fp32 rows' bytes).  A score is the inner product of
     the dequantised rows, summed exactly: |score - <user, item>| <= sum of |u_k| s_i / 2 + |i_k| s_u / 2 + s_u s_i / 4 over k, s = max|row| / 127.
@@ -38,8 +57,9 @@ class CatalogueHead(object):
 
     def draw(self, user_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, residual=None, seen=None):
         """One item a user row -> (ids int32, prob fp32), see ops.sample_rows.  seen: (rows, items) index pair of what is not to
-        be drawn, e.g. the items that a user has rated; a user who has seen everything gets id -1."""
+        be drawn, e.g. the items that a user has rated (a pair outside the scores, such as padding of -1, names nothing); a
+        user who has seen everything gets id -1."""
         s = self.scores(user_rows, residual=residual)
         if seen is not None:
-            s[seen[0].long(), seen[1].long()] = -float("inf")
+            _mask_pairs(s, seen[0], seen[1])
         return ops.sample_rows(s, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)

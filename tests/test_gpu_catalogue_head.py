@@ -773,3 +773,34 @@ def test_distill_bwd_refuses_what_is_not_of_its_forward():
         with pytest.raises(L.StarGCNError):
             ops.distill_bwd(g, s, v, j, 1.0)
             pytest.fail("call %d was not refused" % i)
+
+
+def test_seen_pairs_outside_the_scores_name_nothing():
+    g = gen(14)
+    users, items = torch.randn(5, 32, generator=g).to(DEV), torch.randn(200, 32, generator=g).to(DEV)
+    head = CatalogueHead(items)
+    u = torch.rand(5, generator=g).to(DEV)
+    i64 = lambda v: torch.tensor(v, device=DEV)      # noqa: E731
+    s = head.scores(users)
+    for rows, cols in (([0, 0, 4, 4], [3, 3, 199, 0]), ([0, -1, 5, 1 << 40, 2, 2, 2, 3], [-1, 4, 7, 7, 200, 1 << 40, -(1 << 40), 9]), ([], [])):
+        masked = s.clone()
+        for r, c in zip(rows, cols):
+            if 0 <= r < 5 and 0 <= c < 200:
+                masked[r, c] = -INF
+        seen = (i64(rows).long(), i64(cols).long())
+        for kw in (dict(), dict(top_k=1)):
+            want, got = ops.sample_rows(masked, u, **kw), head.draw(users, u, seen=seen, **kw)
+            assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    best = s.argmax(1)
+    ids, _ = head.draw(users, u, top_k=1, seen=(torch.arange(5, device=DEV).int(), best.int()))
+    assert (ids != best).all()
+    every = (torch.arange(5, device=DEV)[:, None], torch.arange(200, device=DEV))      # every pair
+    ids, prob = head.draw(users, u, seen=every)
+    assert (ids == -1).all() and (prob == 0).all()
+    lost = users.clone()
+    lost[0, 1] = math.nan                                  # scores of NaN stay what is never drawn
+    ids, prob = head.draw(lost, u, seen=(i64([-1, 0]), i64([-1, 2])))
+    assert ids[0] == -1 and (ids[1:] >= 0).all()
+    for bad in ((best, best[:3]), (best, best.float()), (best > 0, best), (best.cpu(), best)):
+        with pytest.raises(L.StarGCNError):
+            head.draw(users, u, seen=bad)
