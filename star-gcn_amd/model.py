@@ -366,6 +366,8 @@ class Net(nn.Module):
                                                graph_sampler_args=graph_sampler_args, symm=symm, device=device,
                                                full_node_ids=full)
             plan["idx"][b]["n_out"] = {k: int(v.shape[0]) for k, v in uniq.items()}
+            if b == nb - 1:
+                plan["out_ids"] = uniq      # the node ids of the encoder's last output, row by row
         plan["input"] = self._embed_plan(req, embed_noise_dict, embed_noise_dict is not None, device)
         plan["gt"] = (self._embed_plan(recon_node_ids_dict, None, False, device)
                       if recon_node_ids_dict is not None else None)
@@ -410,6 +412,7 @@ class Net(nn.Module):
                 if self._use_fea_proj and not self._recon_fea:
                     idx["req_fea"] = dict(ident)
             plan["idx"][b] = idx
+        plan["out_ids"] = dict(dgraph.node_ids_dict)
         plan["input"] = dict(ident)
         plan["gt"] = None
         if self._use_fea_proj:
@@ -467,11 +470,21 @@ class Net(nn.Module):
         return pred_ratings, pred_embeddings, gt
 
     def rating_rows(self, plan):
-        """(user rows, item rows) of the last block's rating projections, one row a node that the plan computes there: a pair's
-        score is the inner product of its two rows.  What a CatalogueHead (star_gcn_amd.recommend) is made of and asked with."""
+        """(user rows, item rows) of the last block's rating projections, one row a node that the plan computes there, in the
+        order of rating_ids(plan): a pair's score is the inner product of its two rows.  What a CatalogueHead
+        (star_gcn_amd.recommend) is made of and asked with."""
         for k, _idx, out in self._encode(plan):
             pass
         return self.rating_user_projs[k](out[self._name_user]), self.rating_item_projs[k](out[self._name_item])
+
+    def rating_ids(self, plan):
+        """(user ids, item ids) of rating_rows(plan)'s rows, int64 on the plan's device.  A plan of rating pairs holds the pairs'
+        nodes alone, ordered by their first occurrence; one of every node (full_node_ids, make_plan_device, a resident plan)
+        holds them in the graph's order."""
+        if any(key not in plan["out_ids"] for key in (self._name_user, self._name_item)):
+            raise ValueError("the plan computes no %r or no %r nodes" % (self._name_user, self._name_item))
+        return tuple(torch.from_numpy(np.asarray(plan["out_ids"][key], dtype=np.int64)).to(plan["device"])
+                     for key in (self._name_user, self._name_item))
 
     def forward(self, graph, rating_node_pairs=None, embed_noise_dict=None, recon_node_ids_dict=None,
                 graph_sampler_args=None, symm=None, device="cuda", rating_targets=None, rating_scale=None):

@@ -804,3 +804,59 @@ def test_seen_pairs_outside_the_scores_name_nothing():
     for bad in ((best, best[:3]), (best, best.float()), (best > 0, best), (best.cpu(), best)):
         with pytest.raises(L.StarGCNError):
             head.draw(users, u, seen=bad)
+
+
+@pytest.mark.parametrize("kind", ["pairs", "full", "resident"])
+def test_network_answers_with_items_of_the_graph(kind):
+    import star_gcn_amd.model as M
+    import star_gcn_amd.synthetic as S
+    from star_gcn_amd.resident import ResidentPlan
+    torch.manual_seed(1)
+    graph, eu, ei, _ = S.make_graph("tiny")
+    net = M.Net(graph, "user", "movie", embed_units=32, agg_units=(32,), out_units=(32,), nblocks=2, use_dae=True).to(DEV).eval()
+    every = net.make_plan(graph, full_node_ids=graph.node_ids_dict, device=DEV)
+    with torch.no_grad():
+        all_users, all_items = net.rating_rows(every)
+    order = np.random.default_rng(5).permutation(eu.size)[:60]       # some of the pairs, in no order
+    pairs = np.stack([eu[order], ei[order]])
+    plan = {"pairs": lambda: net.make_plan(graph, rating_node_pairs=pairs, device=DEV), "full": lambda: every,
+            "resident": lambda: ResidentPlan(net, graph, device=DEV).set_batch(rating_node_pairs=pairs, remove_batch_edges=False)}[kind]()
+    with torch.no_grad():
+        users, items = net.rating_rows(plan)
+    user_ids, item_ids = net.rating_ids(plan)
+    assert user_ids.shape == users.shape[:1] and item_ids.shape == items.shape[:1] and item_ids.dtype == torch.int64
+    if kind == "pairs":
+        assert sorted(item_ids.tolist()) == sorted(set(pairs[1].tolist())) and item_ids.tolist() != sorted(item_ids.tolist())
+        assert sorted(user_ids.tolist()) == sorted(set(pairs[0].tolist()))
+    # the rows are those of the nodes that the ids name: the whole neighbourhood is aggregated either way, only sums' orders differ
+    for rows, ids, ref in ((users, user_ids, all_users), (items, item_ids, all_items)):
+        assert (rows - ref[ids]).abs().max() <= 2e-5 * ref.abs().max()
+    head = CatalogueHead(items, item_ids=item_ids)
+    s = head.scores(users)
+    best = item_ids[s.argmax(1)]
+    u = torch.rand(users.shape[0], device=DEV)
+    rows = torch.arange(users.shape[0], device=DEV)
+    ids, _ = head.draw(users, u, top_k=1)
+    assert ids.dtype == torch.int64 and torch.equal(ids, best)
+    # the best item masked by its id: the second is drawn.  Items that the catalogue lacks, and no items, mask nothing
+    lacking = sorted(set(range(2000)) - set(item_ids.tolist()))[:3]
+    seen = (torch.cat([rows, rows[:3], rows[:1]]), torch.cat([best, torch.tensor(lacking + [-1], device=DEV)]))
+    ids, _ = head.draw(users, u, top_k=1, seen=seen)
+    assert torch.equal(ids, item_ids[s.topk(2, dim=1).indices[:, 1]])
+    every_item = (rows[:, None], item_ids[None].int())
+    ids, prob = head.draw(users, u, seen=every_item)
+    assert (ids == -1).all() and (prob == 0).all()
+
+
+def test_item_ids_are_checked():
+    x = torch.randn(4, 8, device=DEV)
+    ids = torch.tensor([7, 1 << 40, 0, 3], device=DEV)
+    got, _ = CatalogueHead(x, item_ids=ids).draw(x, torch.rand(4, device=DEV), top_k=1, seen=(torch.zeros(1, dtype=torch.int64, device=DEV), ids[1:2]))
+    assert all(v in ids.tolist() for v in got.tolist()) and got[0] != 1 << 40
+    none, prob = CatalogueHead(x[:0], item_ids=ids[:0]).draw(x, torch.rand(4, device=DEV), seen=(ids[:1], ids[:1]))
+    assert none.tolist() == [-1] * 4
+    small, _ = CatalogueHead(x, item_ids=torch.tensor([9, 8, 7, 6], dtype=torch.int32, device=DEV)).draw(x, torch.rand(4, device=DEV))
+    assert small.dtype == torch.int32
+    for bad in (ids[:3], ids.cpu(), ids.float(), ids[None], torch.tensor([1, 2, 2, 3], device=DEV), torch.tensor([1, 2, -2, 3], device=DEV)):
+        with pytest.raises(L.StarGCNError):
+            CatalogueHead(x, item_ids=bad)
