@@ -546,21 +546,27 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         L.require_current_gpu(v)
         if v.is_floating_point() != dtype.is_floating_point or v.dtype == torch.bool:
             raise L.StarGCNError("sample_rows: %s cannot be of %s" % (name, v.dtype))
-        if v.dtype != dtype:
-            v = v.to(dtype) if dtype.is_floating_point else v.clamp(max=0x7fffffff).to(dtype)
+        if v.dtype != dtype:      # whole numbers: below 0 counts as 0, above any number of items as all of them
+            v = v.to(dtype) if dtype.is_floating_point else v.long().clamp(0, 0x7fffffff).to(dtype)
         return 0, _vector(v.expand(rows) if v.dim() == 0 else v, rows, dtype, "sample_rows " + name)
 
     (t, tr), (p, pr), (m, mr) = (setting(v, torch.float32, name) for v, name in
                                  ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
     k, kr = setting(top_k, torch.int32, "top_k")
-    if kr is None and int(k) != k:
-        raise L.StarGCNError("sample_rows: top_k has to be a whole number, got %r" % (k,))
+    if kr is None:
+        try:
+            whole = int(k)
+        except (TypeError, ValueError, OverflowError):
+            whole = None
+        if whole is None or whole != k:
+            raise L.StarGCNError("sample_rows: top_k has to be a whole number, got %r" % (k,))
+        k = max(min(whole, n), -1)      # negative: refused below
     ids = torch.empty((rows,), dtype=torch.int32, device=logits.device)
     prob = torch.empty((rows,), dtype=torch.float32, device=logits.device)
     lib = L.lib()
     wsn = lib.sg_sample_rows_workspace_bytes(rows, n, dt)
     ws = L.scratch(wsn, logits.device)
-    L.check(lib.sg_sample_rows_hip(L.ptr(ids), L.ptr(prob), L.ptr(logits), ld, dt, L.ptr(u), rows, n, float(t), min(int(k), n), float(p),
+    L.check(lib.sg_sample_rows_hip(L.ptr(ids), L.ptr(prob), L.ptr(logits), ld, dt, L.ptr(u), rows, n, float(t), k, float(p),
                                    float(m), L.ptr(tr), L.ptr(kr), L.ptr(pr), L.ptr(mr), L.ptr(ws), wsn, L.stream_ptr()),
             "sg_sample_rows_hip")
     return ids, prob
@@ -570,7 +576,7 @@ def _item_ids(ids):
     """ids as int32; what int32 cannot hold is no item either way."""
     if ids.is_floating_point() or ids.dtype == torch.bool:
         raise L.StarGCNError("distill_loss: ids have to be whole numbers, got %s" % ids.dtype)
-    return L.i32c(ids.clamp(-1, 0x7fffffff) if ids.dtype == torch.int64 else ids)
+    return L.i32c(ids if ids.dtype == torch.int32 else ids.long().clamp(-1, 0x7fffffff))
 
 
 def _distill_shapes(student, teacher, ids):

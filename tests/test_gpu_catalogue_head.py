@@ -860,3 +860,29 @@ def test_item_ids_are_checked():
     for bad in (ids[:3], ids.cpu(), ids.float(), ids[None], torch.tensor([1, 2, 2, 3], device=DEV), torch.tensor([1, 2, -2, 3], device=DEV)):
         with pytest.raises(L.StarGCNError):
             CatalogueHead(x, item_ids=bad)
+
+
+def test_draw_with_top_k_of_every_integer_type():
+    l, u = torch.randn(6, 300, generator=gen(61)).to(DEV), torch.rand(6, generator=gen(62)).to(DEV)
+    k = [0, 1, 5, 100, 127, 64]
+    want = ops.sample_rows(l, u, top_k=torch.tensor(k, dtype=torch.int32, device=DEV))
+    for t in (torch.int8, torch.uint8, torch.int16, torch.int64):
+        got = ops.sample_rows(l, u, top_k=torch.tensor(k, dtype=t, device=DEV))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), t
+    every = ops.sample_rows(l, u)
+    for t, low in ((torch.int64, -(1 << 32) + 5), (torch.int64, -(1 << 63)), (torch.int32, -(1 << 31)), (torch.int8, -128), (torch.int64, 1 << 40)):
+        top_k = torch.full((6,), low, dtype=t, device=DEV)
+        got = ops.sample_rows(l, u, top_k=top_k)
+        assert (top_k == low).all()                        # the caller's tensor stays as it is
+        assert torch.equal(got[0], every[0]) and torch.equal(got[1], every[1]), low
+    for bad in (INF, -INF, math.nan, 2.5, -(1 << 70), -1, "5", None):
+        with pytest.raises(L.StarGCNError):
+            ops.sample_rows(l, u, top_k=bad)
+
+
+def test_distill_ids_of_every_integer_type():
+    s, t = torch.randn(3, 100, generator=gen(63)).to(DEV), torch.randn(3, 4, generator=gen(64)).to(DEV)
+    ids = torch.randint(0, 100, (3, 4), generator=gen(65))
+    want = SF.distill_loss(s, t, ids.int().to(DEV), 1.0)
+    for dt in (torch.int8, torch.uint8, torch.int16, torch.int64):
+        assert torch.equal(SF.distill_loss(s, t, ids.to(dt).to(DEV), 1.0), want), dt
