@@ -687,7 +687,7 @@ int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int64_t ld
  * An id outside [0, n) or a teacher score of -inf is no entry; a row without an entry, or without a student score above -inf,
  * adds no loss and gets a zero gradient.  An item may be named more than once.  The forward leaves stats (rows, 2) and p
  * (rows, k) for the backward; grad (rows, n) is contiguous and of the student's type; grad_loss is one number on the device.
- * Fewer than 2^24 rows and 2^30 items. */
+ * Fewer than 2^24 rows and 2^30 items; 2^-63 <= temperature <= 2^63. */
 #define SG_DISTILL_MAX_K 1024
 size_t sg_distill_workspace_bytes(int64_t rows, int64_t n);
 int sg_distill_hip(float* loss, float* stats, float* p, const void* student, int64_t ld, int dtype, const float* teacher,

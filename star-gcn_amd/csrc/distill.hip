@@ -29,7 +29,7 @@ struct DistillArgs {
   float* stats;            // (rows, 2): largest score, 1 / sum exp (0: the row has nothing to fit)
   float* p;                // (rows, K)
   float* part;             // (rows, splits, 2): running maximum and sum of a piece
-  float* row_loss;         // (rows)
+  float* row_loss;         // (rows): in the scores' unit, T sum p (log p - log q), which is about as large as the scores' differences
   void* grad;
   const float* gout;
   long long ld;
@@ -177,7 +177,7 @@ __device__ __forceinline__ void finish_row(const DistillArgs& g, int row, float 
   if (lane == 0) {
     g.stats[2 * row] = m;
     g.stats[2 * row + 1] = none ? 0.f : 1.f / s;
-    g.row_loss[row] = static_cast<float>(loss);
+    g.row_loss[row] = static_cast<float>(loss * g.temperature);
   }
 }
 
@@ -307,7 +307,8 @@ inline int check_args(const char* what, int dtype, int64_t ld, int64_t rows, int
   if (n >= (1ll << 30) || rows >= (1ll << 24) || k > SG_DISTILL_MAX_K)      // 2^32 threads a launch
     return fail(SG_ERR_UNSUPPORTED, "%s: at most %d teacher entries a row, fewer than 2^24 rows and 2^30 items", what, SG_DISTILL_MAX_K);
   if (ld < n) return fail(SG_ERR_INVALID, "%s: rows overlap", what);
-  if (!(temperature > 0.f) || !(temperature <= 3.402823466e38f)) return fail(SG_ERR_INVALID, "%s: temperature must be positive", what);
+  // beyond, its square leaves 32 bits: the loss's factor, and at the lower end the exponents' too
+  if (!(temperature >= 0x1p-63f) || !(temperature <= 0x1p63f)) return fail(SG_ERR_INVALID, "%s: temperature must lie between 2^-63 and 2^63", what);
   return SG_OK;
 }
 
@@ -347,7 +348,7 @@ SG_API int sg_distill_hip(float* loss, float* stats, float* p, const void* stude
     else run(bf16{});
   }
   hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kSumThreads), 0, st, loss, row_loss, static_cast<int>(rows),
-                     static_cast<double>(scale) * temperature * temperature);
+                     static_cast<double>(scale) * temperature);
   return check_launch("distill");
 }
 

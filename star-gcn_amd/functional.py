@@ -190,5 +190,6 @@ def distill_loss(student, teacher, ids, scale, temperature=1.0):
     """scale * temperature^2 * sum over rows of KL(p || q): p = softmax(teacher / temperature) over the teacher's k best items of
     a row, q = softmax(student / temperature) over all its items.  student (rows, items) fp32 / fp16 / bf16 scores, teacher
     (rows, k) their scores, ids (rows, k) their items.  An id outside the items (-1) or a teacher score of -inf is padding; a row
-    of padding, or with no student score above -inf, adds nothing.  The teacher gets no gradient."""
+    of padding, or with no student score above -inf, adds nothing.  temperature from 2^-63 to 2^63.  The
+    teacher gets no gradient."""
     return _Distill.apply(student, teacher, ids, float(scale), float(temperature))

@@ -80,3 +80,10 @@ def test_host_tensors_are_refused():
                  lambda: ops.gemm_i8(x.char(), x[:, 0], x.char(), x[:, 0]), lambda: SF.distill_loss(x, x, x.int(), 1.0)):
         with pytest.raises(L.StarGCNError):
             call()
+
+
+@pytest.mark.parametrize("temp", [1e-39, 1e-45, 2.0 ** -63.01, 2.0 ** 63.01, 3e38, -1.0, NAN])
+def test_distill_refuses_temperatures_whose_square_leaves_32_bits(temp):
+    assert distill(temp=temp) == -1 and distill_bwd(temp=temp) == -1
+    for t in (2.0 ** -63, 2.0 ** 63):      # the ends themselves pass this check: the next one refuses the missing workspace
+        assert distill(temp=t, ws=None) == -5

@@ -886,3 +886,34 @@ def test_distill_ids_of_every_integer_type():
     want = SF.distill_loss(s, t, ids.int().to(DEV), 1.0)
     for dt in (torch.int8, torch.uint8, torch.int16, torch.int64):
         assert torch.equal(SF.distill_loss(s, t, ids.to(dt).to(DEV), 1.0), want), dt
+
+
+@pytest.mark.parametrize("T", [2.0 ** -63, 1e-10, 1e-3, 0.5, 1e3, 1e10, 2.0 ** 63])
+def test_distill_at_every_temperature(T):
+    g = gen(71)
+    for dtype in DTYPES:
+        s = (2 * torch.randn(6, 333, generator=g)).to(dtype)
+        t = s.float().gather(1, torch.arange(12).expand(6, 12)) + torch.randn(6, 12, generator=g)
+        ids = torch.stack([torch.randperm(333, generator=g)[:12] for _ in range(6)]).int()
+        s[4, 10:40] = -INF
+        s[5] = 0.25                                        # all alike
+        ids[4] = torch.arange(50, 62)
+        if dtype == torch.float16 and T >= 1e10:
+            # scale T q is about 1e10 / 6 / 333 = 5e6: past 65520 the nearest fp16 number is infinity
+            x = s.to(DEV).requires_grad_(True)
+            grad, = torch.autograd.grad(SF.distill_loss(x, t.to(DEV), ids.to(DEV), 1.0 / 6, temperature=T), x)
+            _, want, size = distill_reference(s, t, ids, 1.0 / 6, T)
+            past = want.abs() - T / 6 * 7e-6 * size > 65520
+            assert past.sum() > 1900 and torch.equal(grad.cpu().double()[past], torch.sign(want)[past] * INF) and (grad[4, 10:40] == 0).all()
+            continue
+        check_distill(s, t, ids, scale=1.0 / 6, T=T)
+
+
+@pytest.mark.parametrize("T", [0.3, 0.5, 2.0])
+def test_distill_towards_items_masked_by_the_lowest_value(T):
+    g = gen(72)
+    s, t = torch.randn(4, 200, generator=g), torch.randn(4, 6, generator=g)
+    ids = torch.stack([torch.randperm(200, generator=g)[:6] for _ in range(4)]).int()
+    s[1, ids[1, 2].long()] = -3.4028234663852886e38        # the loss is as large as the score, and finite
+    s[2, ids[2].long()] = -3.4028234663852886e38
+    check_distill(s, t, ids, scale=1.0 / 8, T=T)
