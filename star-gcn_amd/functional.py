@@ -183,7 +183,7 @@ class _Distill(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         student, ids, saved = ctx.saved_tensors
-        return ops.distill_bwd(g, student, saved, ids, ctx.scale, ctx.temperature), None, None, None, None
+        return ops._distill_bwd(g, student, saved, ids, ctx.scale, ctx.temperature), None, None, None, None
 
 
 def distill_loss(student, teacher, ids, scale, temperature=1.0):

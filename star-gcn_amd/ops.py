@@ -610,19 +610,25 @@ def distill_fwd(student, teacher, ids, scale, temperature=1.0):
 def distill_bwd(grad_loss, student, saved, ids, scale, temperature=1.0):
     """The gradient of distill_fwd's loss for the student's scores (contiguous, the student's type).  `saved` and everything else
     as of that call; grad_loss one number."""
-    L.require_current_gpu(grad_loss, student, saved, ids)
     _dtype_id(student, "distill_loss")
+    if student.dim() != 2 or ids.dim() != 2 or ids.shape[0] != student.shape[0]:
+        raise L.StarGCNError("distill_loss: student (rows, items) and ids (rows, k) expected, got %s and %s" %
+                             (tuple(student.shape), tuple(ids.shape)))
+    (rows, n), k = student.shape, ids.shape[1]
+    want = rows * (2 + k) + L.lib().sg_distill_workspace_bytes(rows, n) // 4
+    if saved.dtype != torch.float32 or saved.dim() != 1 or saved.numel() != want or not saved.is_contiguous():
+        raise L.StarGCNError("distill_loss: saved is not of a forward pass over %d rows of %d items with %d entries each" % (rows, n, k))
+    if grad_loss.numel() != 1:
+        raise L.StarGCNError("distill_loss: the loss's gradient is one number, got shape %s" % (tuple(grad_loss.shape),))
+    return _distill_bwd(grad_loss, student, saved, ids, scale, temperature)
+
+
+def _distill_bwd(grad_loss, student, saved, ids, scale, temperature):
+    """distill_bwd of what autograd has kept: shapes are not compared again."""
+    L.require_current_gpu(grad_loss, student, saved, ids)
     student, ld = _rows(student, "distill_loss")
     ids = _item_ids(ids)
     rows, n = student.shape
-    if ids.dim() != 2 or ids.shape[0] != rows:
-        raise L.StarGCNError("distill_loss: ids of shape (%d, k) expected, got %s" % (rows, tuple(ids.shape)))
-    want = rows * (2 + ids.shape[1]) + L.lib().sg_distill_workspace_bytes(rows, n) // 4
-    if saved.dtype != torch.float32 or saved.dim() != 1 or saved.numel() != want or not saved.is_contiguous():
-        raise L.StarGCNError("distill_loss: saved is not of a forward pass over %d rows of %d items with %d entries each" %
-                             (rows, n, ids.shape[1]))
-    if grad_loss.numel() != 1:
-        raise L.StarGCNError("distill_loss: the loss's gradient is one number, got shape %s" % (tuple(grad_loss.shape),))
     grad = torch.empty((rows, n), dtype=student.dtype, device=student.device)
     at = saved.data_ptr()
     L.check(L.lib().sg_distill_bwd_hip(L.ptr(grad), L.ptr(student), ld, L.DTYPE[student.dtype], at, at + 8 * rows, L.ptr(ids), rows, n,
