@@ -917,3 +917,33 @@ def test_distill_towards_items_masked_by_the_lowest_value(T):
     s[1, ids[1, 2].long()] = -3.4028234663852886e38        # the loss is as large as the score, and finite
     s[2, ids[2].long()] = -3.4028234663852886e38
     check_distill(s, t, ids, scale=1.0 / 8, T=T)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["two levels", "few levels", "rising", "falling", "rising, masked"])
+def test_distill_sums_of_long_rows_of_a_large_batch(dtype, kind):
+    # 1024 rows: a row is not split, and a thread adds hundreds of vectors, whose roundings all go the same way where terms repeat
+    rows, n = 1024, 400000
+    g = torch.Generator(device=DEV).manual_seed(3)
+    i = torch.arange(n, device=DEV)
+    row = {"two levels": torch.randint(0, 2, (n,), generator=g, device=DEV), "few levels": torch.randint(0, 50, (n,), generator=g, device=DEV) * 0.1,
+           "rising": (i // 1024) * 1e-4, "falling": 1.0 - (i // 1024) * 1e-4,
+           "rising, masked": ((i // 1024) * 1e-4).masked_fill(i % 3 == 0, -INF)}[kind].to(dtype)
+    s = row.expand(rows, n).contiguous()
+    t, ids = torch.zeros(rows, 4, device=DEV), (torch.arange(4, device=DEV) * 3 + 1).expand(rows, 4).contiguous()
+    x = s.requires_grad_(True)
+    loss = SF.distill_loss(x, t, ids, 1.0 / rows)
+    grad, = torch.autograd.grad(loss, x)
+    z = row.double()
+    q = torch.softmax(z, 0)
+    log_q = torch.log_softmax(z, 0)[ids[0]]
+    # the rows are alike.  A term: exponents up to 4 log2(e), rounded twice (4 * 2^-24 * 2 * ln 2 * 1.45 = 5e-7), v_exp_f32 one step
+    # (1.2e-7); a vector's terms pairwise, three half steps (1.8e-7); the waves' joins and the inverse a few more half steps: 1.5e-6
+    assert abs(loss.item() - (-math.log(4.0) - log_q.mean().item())) <= 1.5e-6 + 2.0 ** -22 * abs(log_q.mean().item())
+    rest = torch.ones(n, dtype=torch.bool, device=DEV)
+    rest[ids[0]] = False
+    fi = torch.finfo(dtype)
+    for r in (0, 511, 1023):
+        # the gradient's own exponent and products as much again, and the type's rounding
+        err = (grad[r].double() * rows - q).abs()[rest]
+        assert (err <= (3e-6 + fi.eps / 2) * q[rest] + rows * fi.smallest_normal * fi.eps).all(), float((err / q[rest]).max())
