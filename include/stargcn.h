@@ -672,6 +672,9 @@ int sg_gemm_i8_hip(void* C, int64_t ldc, int dtype, const int8_t* A, int64_t lda
  * first index at which the kept weight up to it exceeds u[row] times the kept weight, prob[row] = its share.  temperature 0,
  * top_p 0 or min_p > 1 leave the first item.  Scores of -inf and NaN are never drawn; a row of nothing else gets -1 and 0.
  * Settings are scalars, or one a row where the *_rows pointer is not NULL (values below 0 count as 0 there).  u in [0, 1).
+ * A weight is held to 4e-14 of its value, or to half of 2^-s where that is more, s = min(51, 63 - ceil(log2 n)) up to 2^20 items and
+ * 51 above: all items of a row together are off by at most 2^-24 of the first item's weight up to 2^28 items, by 2^-22 at 2^30, and
+ * an item of less than 2^-(s+1) of the first one's weight is not drawn.
  * Rows of more than 16384 items: fewer than 2^23 of them. */
 #define SG_SAMPLE_MAX_ITEMS (1 << 30)
 size_t sg_sample_rows_workspace_bytes(int64_t rows, int64_t n, int dtype);

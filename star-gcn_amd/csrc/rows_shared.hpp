@@ -123,6 +123,9 @@ template <int CTRL, int ROWS, typename T>
 __device__ __forceinline__ T dpp(T v, T rest) {
   if constexpr (sizeof(T) == 4) {
     return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, rest), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else if constexpr (sizeof(T) == 16) {
+    const unsigned long long lo = dpp<CTRL, ROWS>(static_cast<unsigned long long>(v), static_cast<unsigned long long>(rest));
+    return static_cast<T>(dpp<CTRL, ROWS>(static_cast<unsigned long long>(v >> 64), static_cast<unsigned long long>(rest >> 64))) << 64 | lo;
   } else {
     const long long a = __builtin_bit_cast(long long, v), r = __builtin_bit_cast(long long, rest);
     const unsigned lo = __builtin_amdgcn_update_dpp(static_cast<int>(r), static_cast<int>(a), CTRL, ROWS, 0xf, false);
@@ -147,6 +150,8 @@ template <typename T>
 __device__ __forceinline__ T from_lane(T v, int lane) {
   if constexpr (sizeof(T) == 4) {
     return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else if constexpr (sizeof(T) == 16) {
+    return static_cast<T>(from_lane(static_cast<unsigned long long>(v >> 64), lane)) << 64 | from_lane(static_cast<unsigned long long>(v), lane);
   } else {
     const long long a = __builtin_bit_cast(long long, v);
     const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(a), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(a >> 32), lane);

@@ -5,10 +5,12 @@
 //   and min-p (w_i >= m) leave, and at least the first item.
 //   drawn: the first item, by index, at which the kept weight summed up to it exceeds u times the kept weight
 //
-// Which item is drawn is a decision at the border of two sums over the catalogue, so a weight is a whole number: w * 2^s, s =
-// min(51, 62 - log2 N), from a 64-bit polynomial.  Sums of whole numbers are exact in any order: the result does not depend on
-// how the row is spread over threads and workgroups, on the order of the atomic additions, or on the run.  Weights below
-// 2^-(s+1) of the largest are 0 and cannot be drawn.
+// Which item is drawn is a decision at the border of two sums over the catalogue, so a weight is a whole number: w * 2^s, from a
+// 64-bit polynomial.  Sums of whole numbers are exact in any order: the result does not depend on how the row is spread over
+// threads and workgroups, on the order of the atomic additions, or on the run.  Weights below 2^-(s+1) of the largest are 0 and
+// cannot be drawn, so N items can gain or lose N 2^-(s+1) of the largest weight together.  Rows of up to 2^20 items are summed
+// in 64 bits, s = min(51, 63 - log2 N): at most 2^-24, half a step of an fp32 share.  Longer rows keep s = 51 and are summed in
+// 128 bits: 2^-24 up to 2^28 items, 2^-22 at 2^30 (4 x 10,000,000 fp32, no limits: 106 us; in 64 bits 96, which lost 2e-5).
 //
 // The order is never formed.  A histogram of (max l - l) / T, count and weight, shows in which bin a limit falls.  The limit's
 // own element is found among that bin's elements, by rank where they are few, else by subdividing the range of their place in
@@ -39,6 +41,42 @@ constexpr int kMaxPieces = 32, kMaxParts = 128;
 constexpr int kLevels = 4096 / kThreads;      // groups of four that a thread holds of a short row
 
 typedef unsigned long long u64;
+typedef unsigned __int128 u128;
+constexpr int kNarrowItems = 1 << 20;          // rows summed in 64 bits
+
+// sums of weights, at most 2^52 each, from many threads at once: S is u64 or u128 (two atomic additions, the second only where
+// the first has passed 2^64)
+template <typename S, int N>
+struct Sums {
+  u64 v[N];
+  __device__ __forceinline__ u64 get(int i) const { return v[i]; }
+  __device__ __forceinline__ void set(int i, u64 x) { v[i] = x; }
+  __device__ __forceinline__ void add(int i, u64 w) { atomicAdd(&v[i], w); }
+};
+template <int N>
+struct Sums<u128, N> {
+  u64 lo[N];
+  unsigned hi[N];                              // a sum is below 2^82
+  __device__ __forceinline__ u128 get(int i) const { return static_cast<u128>(hi[i]) << 64 | lo[i]; }
+  __device__ __forceinline__ void set(int i, u128 x) { lo[i] = static_cast<u64>(x), hi[i] = static_cast<unsigned>(x >> 64); }
+  __device__ __forceinline__ void add(int i, u64 w) {
+    if (atomicAdd(&lo[i], w) > ~w) atomicAdd(&hi[i], 1u);
+  }
+};
+__device__ __forceinline__ double as_double(u64 v) { return static_cast<double>(v); }
+__device__ __forceinline__ double as_double(u128 v) {
+  return fma(static_cast<double>(static_cast<u64>(v >> 64)), 18446744073709551616.0, static_cast<double>(static_cast<u64>(v)));
+}
+// a whole number that S holds
+template <typename S>
+__device__ __forceinline__ S as_sum(double x) {
+  if constexpr (sizeof(S) == 8) {
+    return static_cast<u64>(x);
+  } else {
+    const u64 hi = static_cast<u64>(x * 5.421010862427522e-20);      // 2^-64
+    return static_cast<u128>(hi) << 64 | static_cast<u64>(fma(static_cast<double>(hi), -18446744073709551616.0, x));
+  }
+}
 
 struct SampleArgs {
   int32_t* ids;
@@ -56,12 +94,12 @@ struct SampleArgs {
   // and, for the passes that leave little behind, parts of `part` items
   int pieces, piece, parts, part, span, chunks, room;
   float* tops;                     // (rows, parts)
-  u64* mass;                       // (rows, pieces, kBins)
+  void* mass;                      // (rows, pieces, kBins) sums
   unsigned* count;
-  struct RowState* state;          // (rows)
+  void* state;                     // (rows) RowState
   unsigned* listed;                // (rows, parts): candidates of the part, which may be more than `room`
   u64* list;                       // (rows, parts, room): their places in the order
-  u64* chunk;                      // (rows, chunks): weight of what is surely kept
+  void* chunk;                     // (rows, chunks) sums: weight of what is surely kept
 };
 
 struct Row {                       // a row's settings, the same on every thread
@@ -76,6 +114,9 @@ struct Row {                       // a row's settings, the same on every thread
 __device__ __forceinline__ u64 uniform(u64 v) {
   return static_cast<u64>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32)))) << 32 |
          static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+}
+__device__ __forceinline__ u128 uniform(u128 v) {
+  return static_cast<u128>(uniform(static_cast<u64>(v >> 64))) << 64 | uniform(static_cast<u64>(v));
 }
 __device__ __forceinline__ double uniform(double v) {
   return __longlong_as_double(static_cast<long long>(uniform(static_cast<u64>(__double_as_longlong(v)))));
@@ -157,42 +198,48 @@ __device__ __forceinline__ u64 whole(double w) {                  // w < 2^52, t
   return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
+template <typename S>
 struct Histogram {
-  u64 mass[kBins];
+  Sums<S, kBins> mass;
   unsigned count[kBins];
 };
 
+template <typename S>
 struct Shared {
-  Histogram hist;                  // of the row, or of a subdivision
+  Histogram<S> hist;               // of the row, or of a subdivision
   bool divided;                    // a subdivision has replaced the row's
   u64 few_place[kFew], few_weight[kFew];
-  u64 wave_a[kWaves], wave_b[kWaves];
-  u64 limit, limit_mass;
+  S wave_a[kWaves];
+  u64 wave_b[kWaves];
+  u64 limit;
+  S limit_mass;
   unsigned few;
   // of find_bin, two in turn: what one call leaves is read while the next one starts
-  u64 before_mass[2];
+  S before_mass[2];
   unsigned before_count[2];
   int found[2];
 };
 
 // sum of the lanes below this one
-__device__ __forceinline__ u64 wave_before(u64 v) {
-  return wave_scan(v, u64{0}, [](u64 a, u64 b) { return a + b; }) - v;
+template <typename S>
+__device__ __forceinline__ S wave_before(S v) {
+  return wave_scan(v, S{0}, [](S a, S b) { return a + b; }) - v;
 }
 
 // The bin, counted from bin 0 on, in which the sum of counts reaches need (by_mass: the sum of weights), need = need_of(total
 // weight), and the sums before it; kBins if there is none.  Two barriers; `turn` is the calls' own count.  Also starts an empty
 // list of candidates.
-template <typename Need>
-__device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, int& turn, bool by_mass, Need need_of, unsigned& before_count,
-                                        u64& before_mass) {
+template <typename S, typename Need>
+__device__ __forceinline__ int find_bin(Shared<S>& sh, const Histogram<S>& h, int& turn, bool by_mass, Need need_of,
+                                        unsigned& before_count, S& before_mass) {
   const int t = threadIdx.x, wave = t / kWave, lane = t % kWave, k = turn++ & 1;
   if (t == 0) sh.found[k] = kBins, sh.before_count[k] = 0, sh.before_mass[k] = 0, sh.few = 0;
-  u64 m[kPer], ms = 0;
+  S m[kPer], ms = 0;
   unsigned c[kPer], cs = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) m[i] = h.mass[kPer * t + i], c[i] = h.count[kPer * t + i], ms += m[i], cs += c[i];
-  u64 mb = wave_before(ms), cb = wave_before(u64{cs}), total = 0;
+  for (int i = 0; i < kPer; ++i) m[i] = h.mass.get(kPer * t + i), c[i] = h.count[kPer * t + i], ms += m[i], cs += c[i];
+  S mb = wave_before(ms), total = 0;
+  u64 cb = wave_before(u64{cs});
   if (lane == kWave - 1) sh.wave_a[wave] = mb + ms, sh.wave_b[wave] = cb + cs;
   __syncthreads();
 #pragma unroll
@@ -200,10 +247,10 @@ __device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, int& tur
     total += sh.wave_a[i];
     if (i < wave) mb += sh.wave_a[i], cb += sh.wave_b[i];
   }
-  const u64 need = need_of(uniform(total));
+  const S need = need_of(uniform(total));
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const u64 a = by_mass ? mb : cb, v = by_mass ? m[i] : c[i];
+    const S a = by_mass ? mb : S{cb}, v = by_mass ? m[i] : S{c[i]};
     if (a < need && need <= a + v) sh.found[k] = kPer * t + i, sh.before_count[k] = static_cast<unsigned>(cb), sh.before_mass[k] = mb;
     mb += m[i], cb += c[i];
   }
@@ -212,49 +259,52 @@ __device__ __forceinline__ int find_bin(Shared& sh, const Histogram& h, int& tur
   return __builtin_amdgcn_readfirstlane(sh.found[k]);
 }
 
-__device__ __forceinline__ void clear(Histogram& h) {              // a barrier has to follow
-  for (int i = threadIdx.x; i < kBins; i += kThreads) h.mass[i] = 0, h.count[i] = 0;
+template <typename S>
+__device__ __forceinline__ void clear(Histogram<S>& h) {           // a barrier has to follow
+  for (int i = threadIdx.x; i < kBins; i += kThreads) h.mass.set(i, 0), h.count[i] = 0;
 }
 
 // a cleared histogram
-template <typename Src>
-__device__ __forceinline__ void fill(Histogram& h, const Src& src, const Scale& sc, bool counts, bool masses) {
+template <typename S, typename Src>
+__device__ __forceinline__ void fill(Histogram<S>& h, const Src& src, const Scale& sc, bool counts, bool masses) {
   src([&](float l, int) {
     const double d = sc.below(l);
     if (!sc.live(d)) return;
     const int b = sc.bin(d);
     if (counts) atomicAdd(&h.count[b], 1u);
-    if (masses) atomicAdd(&h.mass[b], whole(sc.weight(d)));
+    if (masses) h.mass.add(b, whole(sc.weight(d)));
   });
   __syncthreads();
 }
 
 // total weight of a histogram, on every thread
-__device__ __forceinline__ u64 total_mass(Shared& sh, const Histogram& h) {
-  u64 v = 0;
+template <typename S>
+__device__ __forceinline__ S total_mass(Shared<S>& sh, const Histogram<S>& h) {
+  S v = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) v += h.mass[kPer * threadIdx.x + i];
+  for (int i = 0; i < kPer; ++i) v += h.mass.get(kPer * threadIdx.x + i);
   v = wave_sum(v);
   if (threadIdx.x % kWave == 0) sh.wave_a[threadIdx.x / kWave] = v;
   __syncthreads();
-  u64 s = 0;
+  S s = 0;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) s += sh.wave_a[i];
   __syncthreads();
   return uniform(s);
 }
 
-__device__ __forceinline__ u64 share(double p, u64 total) {        // the weight that top-p asks for
-  const u64 need = uniform(static_cast<u64>(ceil(p * static_cast<double>(total))));
-  return min(max(need, u64{1}), total);
+template <typename S>
+__device__ __forceinline__ S share(double p, S total) {            // the weight that top-p asks for
+  const S need = uniform(as_sum<S>(ceil(p * as_double(total))));
+  return need < 1 ? S{1} : need < total ? need : total;
 }
 
 // The limit among the live items of `src` in bins lo_bin .. hi_bin, before which `count` items of weight `mass` stand in the
 // order: by count, the item with which the count reaches `need`; by mass, the item with which the weight does.  -> its place;
 // mass: with the item itself (by count only where `masses`).  The list of candidates is empty.
-template <typename Src>
-__device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, bool by_mass, bool masses,
-                                          u64 need, unsigned count, u64& mass, int& turn) {
+template <typename S, typename Src>
+__device__ __forceinline__ u64 find_limit(Shared<S>& sh, const Src& src, const Scale& sc, int lo_bin, int hi_bin, bool by_mass, bool masses,
+                                          S need, unsigned count, S& mass, int& turn) {
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   u64 lo = 0, hi = ~u64{0};
   auto members = [&](auto f) {
@@ -283,8 +333,8 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
       }
       if (lane == 0) sh.wave_a[wave] = least, sh.wave_b[wave] = most;
       __syncthreads();
-      lo = sh.wave_a[0], hi = sh.wave_b[0];
-      for (int i = 1; i < kWaves; ++i) lo = min(lo, sh.wave_a[i]), hi = max(hi, sh.wave_b[i]);
+      lo = static_cast<u64>(sh.wave_a[0]), hi = sh.wave_b[0];
+      for (int i = 1; i < kWaves; ++i) lo = min(lo, static_cast<u64>(sh.wave_a[i])), hi = max(hi, sh.wave_b[i]);
       lo = uniform(lo), hi = uniform(hi);
     }
     // all places differ: a turn leaves at most 1 / 1024 of the range, and single places at last
@@ -295,13 +345,13 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
     members([&](u64 at, double d) {
       const int digit = static_cast<int>((hi - at) >> shift);
       if (!by_mass) atomicAdd(&sh.hist.count[digit], 1u);
-      if (masses) atomicAdd(&sh.hist.mass[digit], whole(sc.weight(d)));
+      if (masses) sh.hist.mass.add(digit, whole(sc.weight(d)));
     });
     __syncthreads();
     unsigned bc;
-    u64 bm;
-    const u64 rest = need - (by_mass ? mass : count);
-    const int digit = min(find_bin(sh, sh.hist, turn, by_mass, [&](u64) { return rest; }, bc, bm), kBins - 1);
+    S bm;
+    const S rest = need - (by_mass ? mass : S{count});
+    const int digit = min(find_bin(sh, sh.hist, turn, by_mass, [&](S) { return rest; }, bc, bm), kBins - 1);
     count += bc, mass += bm;
     hi -= static_cast<u64>(digit) << shift;
     lo = max(lo, hi - ((u64{1} << shift) - 1));
@@ -319,7 +369,8 @@ __device__ __forceinline__ u64 find_limit(Shared& sh, const Src& src, const Scal
       if (sh.few_place[j] > at) cb += 1, mb += sh.few_weight[j];
   for (int off = 1; off < team; off <<= 1) cb += __shfl_xor(cb, off), mb += __shfl_xor(mb, off);
   if (me < m && t % team == 0) {
-    const u64 w = sh.few_weight[me], before = by_mass ? mass + mb : count + cb, own = by_mass ? w : 1;
+    const u64 w = sh.few_weight[me];
+    const S before = by_mass ? mass + mb : S{count + cb}, own = by_mass ? w : 1;
     if (before < need && need <= before + own) sh.limit = at, sh.limit_mass = mass + mb + w;
   }
   __syncthreads();
@@ -335,20 +386,21 @@ __device__ __forceinline__ u64 kept(float l, int i, const Scale& sc, u64 limit, 
   return w >= min_weight ? whole(w) : 0;
 }
 
-__device__ __forceinline__ u64 goal_of(float u, u64 total) {       // drawn: the first item with more than this up to it
+template <typename S>
+__device__ __forceinline__ S goal_of(float u, S total) {           // drawn: the first item with more than this up to it
   const double x = u;
-  const u64 goal = x > 0.0 ? static_cast<u64>(fmin(x, 1.0) * static_cast<double>(total)) : 0;
-  return min(goal, total - 1);
+  const S goal = x > 0.0 ? as_sum<S>(fmin(x, 1.0) * as_double(total)) : S{0};
+  return goal < total ? goal : total - 1;
 }
 
 // The wave's V items a lane, kept weights w: where the sum from `before` on passes `goal`, that lane writes the item.  -> whether
 // some lane did; before is moved on.
-template <int V>
-__device__ __forceinline__ bool draw(const SampleArgs& g, int row, int base, const u64 (&w)[V], u64 goal, u64 total, u64& before) {
-  u64 sum = 0;
+template <int V, typename S>
+__device__ __forceinline__ bool draw(const SampleArgs& g, int row, int base, const u64 (&w)[V], S goal, S total, S& before) {
+  u64 sum = 0;                                           // 64 lanes of at most 8 weights: below 2^61
 #pragma unroll
   for (int j = 0; j < V; ++j) sum += w[j];
-  u64 b = before + wave_before(sum);
+  S b = before + wave_before(sum);
   const bool hit = b <= goal && goal < b + sum;
   if (hit) {
     bool done = false;
@@ -356,7 +408,7 @@ __device__ __forceinline__ bool draw(const SampleArgs& g, int row, int base, con
     for (int j = 0; j < V; ++j) {
       if (!done && goal < b + w[j]) {
         g.ids[row] = base + j;
-        g.prob[row] = static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total));
+        g.prob[row] = static_cast<float>(static_cast<double>(w[j]) / as_double(total));
         done = true;
       }
       b += w[j];
@@ -382,7 +434,7 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 // not its barriers (eleven instead of twenty: 16.4 -> 15.9 us for 10677 items).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g) {
-  __shared__ Shared sh;
+  __shared__ Shared<u64> sh;
   __shared__ float red[kWaves];
   __shared__ u64 part[kLevels * kWaves];
   extern __shared__ __attribute__((aligned(16))) char lds_row[];
@@ -474,8 +526,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g
 
 // ---- long rows ----------------------------------------------------------------------------------------------------------------
 
+template <typename S>
 struct RowState {
-  u64 total, k_mass, p_mass;       // weight of the row; before the top-k bin; before the top-p bins
+  S total, k_mass, p_mass;         // weight of the row; before the top-k bin; before the top-p bins
   unsigned k_count;                // items before the top-k bin
   int k_bin, p_lo, p_hi;           // kBins: no such limit
 };
@@ -520,9 +573,9 @@ __device__ __forceinline__ float row_top(const SampleArgs& g, int row) {
   return wave_max(top);
 }
 
-template <typename T>
+template <typename T, typename S>
 __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const SampleArgs g) {
-  __shared__ Histogram hist;
+  __shared__ Histogram<S> hist;
   const int row = blockIdx.x / g.pieces, z = blockIdx.x % g.pieces, lo = z * g.piece, hi = min(g.n, lo + g.piece);
   const Row r = row_settings(g, row);
   if (!(r.k > 0 || r.by_p)) return;
@@ -530,31 +583,38 @@ __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const Sample
   __syncthreads();
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   fill(hist, [&](auto f) { each(l, lo, hi, f); }, scale_of(row_top(g, row), r, g.bits), r.k > 0, r.by_p);
-  u64* mass = g.mass + static_cast<long long>(blockIdx.x) * kBins;
+  S* mass = static_cast<S*>(g.mass) + static_cast<long long>(blockIdx.x) * kBins;
   unsigned* count = g.count + static_cast<long long>(blockIdx.x) * kBins;
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    if (r.by_p) mass[i] = hist.mass[i];
+    if (r.by_p) mass[i] = hist.mass.get(i);
     if (r.k > 0) count[i] = hist.count[i];
   }
 }
 
+template <typename S>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs g) {
-  __shared__ Shared sh;
-  Histogram& hist = sh.hist;
+  __shared__ Shared<S> sh;
+  Histogram<S>& hist = sh.hist;
   const int row = blockIdx.x, t = threadIdx.x;
   const Row r = row_settings(g, row);
-  RowState s{0, 0, 0, 0, kBins, kBins, kBins};
+  RowState<S> s{0, 0, 0, 0, kBins, kBins, kBins};
   if (r.k > 0 || r.by_p) {
     static_assert(kPer == 4, "16 bytes of counts a thread");
     const long long at = static_cast<long long>(row) * g.pieces * kBins + kPer * t;      // this thread's bins
-    u64 m[kPer] = {};
+    S m[kPer] = {};
     unsigned c[kPer] = {};
     if (r.by_p) {
 #pragma unroll 8
       for (int z = 0; z < g.pieces; ++z) {
-        const ulonglong2* p = reinterpret_cast<const ulonglong2*>(g.mass + at + static_cast<long long>(z) * kBins);
-        const ulonglong2 a = p[0], b = p[1];
-        m[0] += a.x, m[1] += a.y, m[2] += b.x, m[3] += b.y;
+        const S* piece = static_cast<const S*>(g.mass) + at + static_cast<long long>(z) * kBins;
+        if constexpr (sizeof(S) == 8) {
+          const ulonglong2* p = reinterpret_cast<const ulonglong2*>(piece);
+          const ulonglong2 a = p[0], b = p[1];
+          m[0] += a.x, m[1] += a.y, m[2] += b.x, m[3] += b.y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) m[i] += piece[i];
+        }
       }
     }
     if (r.k > 0) {
@@ -565,30 +625,32 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
       }
     }
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) hist.mass[kPer * t + i] = m[i], hist.count[kPer * t + i] = c[i];
+    for (int i = 0; i < kPer; ++i) hist.mass.set(kPer * t + i, m[i]), hist.count[kPer * t + i] = c[i];
     __syncthreads();
     int turn = 0;
-    u64 most = 0, least = 0;                             // the weight of the top-k items lies between them
+    S most = 0, least = 0;                               // the weight of the top-k items lies between them
     if (r.by_p) least = most = s.total = total_mass(sh, hist);
     if (r.k > 0) {
-      s.k_bin = find_bin(sh, hist, turn, false, [&](u64) { return static_cast<u64>(r.k); }, s.k_count, s.k_mass);
-      if (s.k_bin < kBins) least = s.k_mass, most = s.k_mass + hist.mass[s.k_bin];
+      s.k_bin = find_bin(sh, hist, turn, false, [&](S) { return static_cast<S>(r.k); }, s.k_count, s.k_mass);
+      if (s.k_bin < kBins) least = s.k_mass, most = s.k_mass + hist.mass.get(s.k_bin);
     }
     if (r.by_p && s.total > 0) {                         // no total: a row of nothing but -inf and NaN
       unsigned c;
-      u64 m;
-      s.p_hi = find_bin(sh, hist, turn, true, [&](u64) { return share(r.p, most); }, c, m);
-      s.p_lo = least > 0 ? find_bin(sh, hist, turn, true, [&](u64) { return share(r.p, least); }, c, s.p_mass) : 0;
+      S m;
+      s.p_hi = find_bin(sh, hist, turn, true, [&](S) { return share(r.p, most); }, c, m);
+      s.p_lo = least > 0 ? find_bin(sh, hist, turn, true, [&](S) { return share(r.p, least); }, c, s.p_mass) : 0;
     }
   }
-  if (t == 0) g.state[row] = s;
+  if (t == 0) static_cast<RowState<S>*>(g.state)[row] = s;
 }
 
-__device__ __forceinline__ bool surely_kept(const RowState& s, int bin) { return bin < s.k_bin && bin < s.p_lo; }
-__device__ __forceinline__ bool candidate(const RowState& s, int bin) { return bin == s.k_bin || (bin >= s.p_lo && bin <= s.p_hi); }
+template <typename S>
+__device__ __forceinline__ bool surely_kept(const RowState<S>& s, int bin) { return bin < s.k_bin && bin < s.p_lo; }
+template <typename S>
+__device__ __forceinline__ bool candidate(const RowState<S>& s, int bin) { return bin == s.k_bin || (bin >= s.p_lo && bin <= s.p_hi); }
 
 // one wave a chunk of the part
-template <typename T>
+template <typename T, typename S>
 __global__ __launch_bounds__(256) void sample_parts_kernel(const SampleArgs g) {
   __shared__ unsigned listed;
   constexpr int V = 16 / sizeof(T), U = 4;
@@ -597,14 +659,14 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const SampleArgs g) {
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
   const Row r = row_settings(g, row);
   const Scale sc = scale_of(row_top(g, row), r, g.bits);
-  RowState s{0, 0, 0, 0, kBins, kBins, kBins};
-  if (r.k > 0 || r.by_p) s = g.state[row];
+  RowState<S> s{0, 0, 0, 0, kBins, kBins, kBins};
+  if (r.k > 0 || r.by_p) s = static_cast<const RowState<S>*>(g.state)[row];
   u64* list = g.list + static_cast<long long>(blockIdx.x) * g.room;
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
   const int c0 = z * (g.part / g.span), c1 = min(g.chunks, c0 + g.part / g.span);
   for (int ch = c0 + wave; ch < c1; ch += 4) {
-    u64 sum = 0;
+    u64 sum = 0;                                         // of a lane: at most 4096 items of a chunk, so below 2^64
     const int end = min(g.n, (ch + 1) * g.span);
     auto item = [&](float x, int i) {
       const double d = sc.below(x);
@@ -635,17 +697,18 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const SampleArgs g) {
         for (int j = 0; j < V; ++j)
           if (base + j < end) item(to_f32(l[base + j]), base + j);
     }
-    sum = wave_sum(sum);
-    if (lane == 0) g.chunk[static_cast<long long>(row) * g.chunks + ch] = sum;
+    const S all = wave_sum(S{sum});
+    if (lane == 0) static_cast<S*>(g.chunk)[static_cast<long long>(row) * g.chunks + ch] = all;
   }
   __syncthreads();
   if (threadIdx.x == 0) g.listed[blockIdx.x] = listed;
 }
 
-template <typename T>
+template <typename T, typename S>
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs g) {
-  __shared__ Shared sh;
-  __shared__ u64 chunk[kChunks], lds_list[kListed];
+  __shared__ Shared<S> sh;
+  __shared__ Sums<S, kChunks> chunk;
+  __shared__ u64 lds_list[kListed];
   constexpr int V = 16 / sizeof(T);
   const int row = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / kWave), lane = t % kWave;
   const T* l = static_cast<const T*>(g.l) + row * g.ld;
@@ -656,9 +719,9 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     return;
   }
   const Scale sc = scale_of(top, r, g.bits);
-  RowState s{0, 0, 0, 0, kBins, kBins, kBins};
-  if (r.k > 0 || r.by_p) s = g.state[row];
-  for (int i = t; i < g.chunks; i += kThreads) chunk[i] = g.chunk[static_cast<long long>(row) * g.chunks + i];
+  RowState<S> s{0, 0, 0, 0, kBins, kBins, kBins};
+  if (r.k > 0 || r.by_p) s = static_cast<const RowState<S>*>(g.state)[row];
+  for (int i = t; i < g.chunks; i += kThreads) chunk.set(i, static_cast<const S*>(g.chunk)[static_cast<long long>(row) * g.chunks + i]);
   u64 limit = 0;
   if (s.k_bin < kBins || s.p_lo < kBins) {
     // the parts' lists, one behind the other in LDS if they fit
@@ -676,16 +739,16 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     whole_list = whole_list && listed <= kListed;
     auto limits = [&](auto src) {
       int turn = 0;
-      u64 total = s.total;
+      S total = s.total;
 #pragma unroll 1
       for (int by_mass = 0; by_mass < 2; ++by_mass) {    // top-k, then top-p
         if ((by_mass ? s.p_lo : s.k_bin) == kBins) continue;
-        u64 mass = by_mass ? s.p_mass : s.k_mass;
+        S mass = by_mass ? s.p_mass : s.k_mass;
         __syncthreads();
         if (t == 0) sh.few = 0;
         __syncthreads();
         limit = max(limit, find_limit(sh, src, sc, by_mass ? s.p_lo : s.k_bin, by_mass ? s.p_hi : s.k_bin, by_mass, r.by_p,
-                                      by_mass ? share(r.p, total) : static_cast<u64>(r.k), s.k_count, mass, turn));
+                                      by_mass ? share(r.p, total) : static_cast<S>(r.k), s.k_count, mass, turn));
         total = mass;
       }
     };
@@ -700,7 +763,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       limits(src);
       src([&](float x, int i) {
         const u64 w = kept(x, i, sc, limit, r.m);
-        if (w) atomicAdd(&chunk[i / g.span], w);
+        if (w) chunk.add(i / g.span, w);
       });
     } else {                                             // too many candidates for the list: over the row itself
       limits([&](auto f) { each(l, 0, g.n, f); });
@@ -715,8 +778,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
           for (int j = 0; j < V; ++j)
             if (base + j < end) sum += kept(x[j], base + j, sc, limit, r.m);
         }
-        sum = wave_sum(sum);
-        if (lane == 0) chunk[ch] = sum;
+        const S all = wave_sum(S{sum});
+        if (lane == 0) chunk.set(ch, all);
       }
     }
   }
@@ -724,13 +787,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   if (wave != 0) return;
   // the chunk, then the item, at which the sum passes the drawn share
   const int per = (g.chunks + kWave - 1) / kWave, c0 = min(g.chunks, lane * per), c1 = min(g.chunks, c0 + per);
-  u64 mine = 0;
-  for (int i = c0; i < c1; ++i) mine += chunk[i];
-  const u64 total = wave_sum(mine), goal = goal_of(g.u[row], total);
-  u64 before = wave_before(mine);
+  S mine = 0;
+  for (int i = c0; i < c1; ++i) mine += chunk.get(i);
+  const S total = wave_sum(mine), goal = goal_of(g.u[row], total);
+  S before = wave_before(mine);
   int at = -1;
   if (before <= goal && goal < before + mine)
-    for (at = c0; before + chunk[at] <= goal; ++at) before += chunk[at];
+    for (at = c0; before + chunk.get(at) <= goal; ++at) before += chunk.get(at);
   const int owner = __ffsll(static_cast<unsigned long long>(__ballot(at >= 0))) - 1;
   at = __builtin_amdgcn_readlane(at, owner);
   before = from_lane(before, owner);
@@ -748,6 +811,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
 
 // items of a row that one workgroup holds
 constexpr int kRowItems = kLevels * kThreads * 4;
+static_assert(kRowItems <= kNarrowItems, "short rows are summed in 64 bits");
 
 // long rows: the workspace, from `base` on (null: its size alone)
 inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* base) {
@@ -766,19 +830,35 @@ inline size_t lay_out(SampleArgs& g, int64_t rows, int64_t n, int size, char* ba
   cut(kMaxParts, g.parts, g.part);
   g.room = std::min(kListed, g.part / 4);
   size_t at = 0;
-  auto take = [&](auto*& p, size_t count) {
+  auto take_bytes = [&](auto*& p, size_t bytes) {
     p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
-    at += (count * sizeof(*p) + 255) & ~size_t{255};
+    at += (bytes + 255) & ~size_t{255};
   };
+  auto take = [&](auto*& p, size_t count) { take_bytes(p, count * sizeof(*p)); };
   const size_t pieces = static_cast<size_t>(rows) * g.pieces, parts = static_cast<size_t>(rows) * g.parts;
   take(g.tops, parts);
-  take(g.mass, pieces * kBins);
+  const bool narrow = n <= kNarrowItems;
+  const size_t sum = narrow ? sizeof(u64) : sizeof(u128);
+  take_bytes(g.mass, pieces * kBins * sum);
   take(g.count, pieces * kBins);
-  take(g.state, rows);
+  take_bytes(g.state, rows * (narrow ? sizeof(RowState<u64>) : sizeof(RowState<u128>)));
   take(g.listed, parts);
   take(g.list, parts * g.room);
-  take(g.chunk, static_cast<size_t>(rows) * g.chunks);
+  take_bytes(g.chunk, static_cast<size_t>(rows) * g.chunks * sum);
   return at;
+}
+
+template <typename T, typename S>
+void launch_long(const SampleArgs& g, bool limits, hipStream_t st) {
+  const dim3 block(kThreads), rows(static_cast<unsigned>(g.rows)), pieces(static_cast<unsigned>(g.rows) * g.pieces),
+      parts(static_cast<unsigned>(g.rows) * g.parts);
+  hipLaunchKernelGGL(sample_top_kernel<T>, parts, dim3(256), 0, st, g);
+  if (limits) {
+    hipLaunchKernelGGL((sample_histogram_kernel<T, S>), pieces, block, 0, st, g);
+    hipLaunchKernelGGL(sample_bins_kernel<S>, rows, block, 0, st, g);
+  }
+  hipLaunchKernelGGL((sample_parts_kernel<T, S>), parts, dim3(256), 0, st, g);
+  hipLaunchKernelGGL((sample_draw_kernel<T, S>), rows, block, 0, st, g);
 }
 
 template <typename T>
@@ -798,15 +878,10 @@ void launch(const SampleArgs& g, bool limits, hipStream_t st) {
       if (g.min_p) a.min_p += r;
       hipLaunchKernelGGL(sample_row_kernel<T>, dim3(static_cast<unsigned>(a.rows)), block, lds, st, a);
     }
+  } else if (g.n <= kNarrowItems) {
+    launch_long<T, u64>(g, limits, st);
   } else {
-    const dim3 rows(static_cast<unsigned>(g.rows)), pieces(static_cast<unsigned>(g.rows) * g.pieces), parts(static_cast<unsigned>(g.rows) * g.parts);
-    hipLaunchKernelGGL(sample_top_kernel<T>, parts, dim3(256), 0, st, g);
-    if (limits) {
-      hipLaunchKernelGGL(sample_histogram_kernel<T>, pieces, block, 0, st, g);
-      hipLaunchKernelGGL(sample_bins_kernel, rows, block, 0, st, g);
-    }
-    hipLaunchKernelGGL(sample_parts_kernel<T>, parts, dim3(256), 0, st, g);
-    hipLaunchKernelGGL(sample_draw_kernel<T>, rows, block, 0, st, g);
+    launch_long<T, u128>(g, limits, st);
   }
 }
 
@@ -846,7 +921,7 @@ SG_API int sg_sample_rows_hip(int32_t* ids, float* prob, const void* logits, int
   g.ids = ids, g.prob = prob, g.l = logits, g.u = u;
   g.temperature = temperature_rows, g.top_k = top_k_rows, g.top_p = top_p_rows, g.min_p = min_p_rows;
   g.t0 = temperature, g.p0 = top_p, g.m0 = min_p, g.k0 = top_k;
-  g.ld = ld, g.rows = static_cast<int>(rows), g.n = static_cast<int>(n), g.bits = std::min(51, 62 - log_n);
+  g.ld = ld, g.rows = static_cast<int>(rows), g.n = static_cast<int>(n), g.bits = n <= kNarrowItems ? std::min(51, 63 - log_n) : 51;
   if (long_rows) lay_out(g, rows, n, size, static_cast<char*>(workspace));
   // whether any row can have a limit: otherwise the histogram has no reader
   const bool limits = top_k_rows || top_p_rows || temperature_rows || min_p_rows || (top_k > 0 && top_k < n) || top_p < 1.0 ||

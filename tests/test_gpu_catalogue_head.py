@@ -947,3 +947,71 @@ def test_distill_sums_of_long_rows_of_a_large_batch(dtype, kind):
         # the gradient's own exponent and products as much again, and the type's rounding
         err = (grad[r].double() * rows - q).abs()[rest]
         assert (err <= (3e-6 + fi.eps / 2) * q[rest] + rows * fi.smallest_normal * fi.eps).all(), float((err / q[rest]).max())
+
+
+def peak_and_tail(n, x, dtype, peak):
+    """One score of 0 and n - 1 of x -> scores, the weight of a tail item and of all (the peak's is 1), what the tail's weights may be
+    off by together: half a unit of their fixed point each."""
+    l = torch.full((1, n), x, dtype=dtype, device=DEV)
+    l[0, peak] = 0.0
+    w = math.exp(float(l[0, (peak + 1) % n]))
+    unit = max(63 - math.ceil(math.log2(n)), 0) if n <= 1 << 20 else 51
+    return l, w, 1.0 + (n - 1) * w, n * 2.0 ** -(min(unit, 51) + 1)
+
+
+@pytest.mark.parametrize("n,x,dtype", [(1 << 20, -25.0, torch.float32), (1 << 20, -31.0, torch.float32), ((1 << 20) + 1, -31.0, torch.float32),
+                                       (10000000, -27.0, torch.float32), (10000000, -27.2, torch.float32), (10000000, -16.0, torch.float16),
+                                       (1 << 26, -26.0, torch.bfloat16), (1 << 28, -24.25, torch.bfloat16), (1 << 28, -19.0, torch.float16)])
+def test_draw_of_a_flat_tail_that_holds_what_one_unit_of_weight_does_not(n, x, dtype):
+    peak = n // 3
+    l, w, total, off = peak_and_tail(n, x, dtype, peak)
+    assert off <= 2.0 ** -24 * 1.01
+    first, last = peak * w / total, (peak * w + 1.0) / total      # the shares between which the peak is drawn
+    margin = off / total + 2.0 ** -24                      # and u itself is rounded to fp32
+    us = [first / 2, first + 1.5 * margin, 0.5 * (first + last), last - 1.5 * margin, 0.5 * (1.0 + last)]
+    want = [first > 4 * margin, True, True, True, 1 - last > 4 * margin]
+    for u, sure, inside in zip(us, want, (False, True, True, True, False)):
+        if not sure:
+            continue
+        ids, prob = ops.sample_rows(l, torch.tensor([u], device=DEV))
+        assert (ids.item() == peak) == inside, (u, ids.item())
+        if inside:
+            assert abs(prob.item() - 1.0 / total) <= off / total + 2.0 ** -24
+        else:
+            # an item of the tail, as far along as u asks for: its weight is off by half a unit
+            assert 0 <= ids.item() < n and abs(prob.item() - w / total) <= 2 * off / n + 2.0 ** -24 * w / total
+            at = float(np.float32(u)) * total / w
+            if u > last:
+                at = (float(np.float32(u)) * total - 1.0) / w + 1
+            assert abs(ids.item() - at) <= 2 * off / w + 2 + n * 1e-9
+
+
+@pytest.mark.parametrize("n", [(1 << 20) + 1, 3000000, 10000000])
+def test_draw_among_millions_of_equal_scores(n):
+    # the weight of all of them passes 2^64; ranks and shares are known without a sum
+    l = torch.zeros(4, n, device=DEV, dtype=torch.float16)
+    l[1] = 1.5
+    l[1, n // 2:] = -INF
+    l[2, ::2] = math.nan
+    l[3, 7] = INF
+    u = torch.tensor([0.75, 0.75, 0.75, 0.75], device=DEV)
+    live = [n, n // 2, n // 2, 1]
+    index = [lambda r: r, lambda r: r, lambda r: 2 * r + 1, lambda r: 7]
+    for kw, keep in ((dict(), lambda m: m), (dict(top_k=1000001), lambda m: min(m, 1000001)), (dict(top_p=0.5), lambda m: math.ceil(m * 0.5)),
+                     (dict(top_k=600000, top_p=0.25), lambda m: math.ceil(min(m, 600000) * 0.25)), (dict(min_p=1.0), lambda m: m)):
+        ids, prob = ops.sample_rows(l, u, **kw)
+        for i in range(4):
+            m = keep(live[i])
+            assert ids[i].item() == index[i](int(0.75 * m)), (kw, i)
+            assert abs(prob[i].item() * m - 1) <= 2.0 ** -23, (kw, i)
+
+
+@pytest.mark.parametrize("n,dtype", [(1 << 20, torch.float32), ((1 << 20) + 1, torch.float32), (3000001, torch.bfloat16), (3000000, torch.float32)])
+def test_draw_from_rows_of_millions(n, dtype):
+    g = gen(n)
+    l = torch.randn(3, n, generator=g).to(dtype)
+    l[1] = (0.3 * torch.randn(n, generator=g)).to(dtype)
+    l[2, torch.rand(n, generator=g) < 0.5] = -INF
+    u = torch.rand(3, generator=g)
+    for kw in (dict(), dict(top_p=0.95), dict(top_k=700), dict(top_k=40000, top_p=0.7, min_p=1e-3), dict(min_p=0.01, temperature=0.5)):
+        check_draw(l, u, **kw)
