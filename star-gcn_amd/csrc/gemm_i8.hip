@@ -4,7 +4,8 @@
 //
 // B holds one output channel a row (an item's row, a dense layer's weight as it is stored).  The sums are exact in 32-bit
 // integers (K < 2^17), so every kernel and every split of K gives the same bits; the epilogue rounds the sum to fp32, its product
-// with sa, the fused product with sb and bias, and the result to C's type.
+// with sa, the fused product with sb and bias, and the result to C's type.  The product of the three is right over fp32's whole
+// range: waves in which some sa is 2^97 or more, or below the normal numbers, take a path of their own.
 //
 // Tile kernel.  v_mfma_i32_32x32x32_i8: a lane feeds 16 consecutive k of one row of A and one of B, so both operands are used
 // exactly as they lie in memory.  A K step is 64 or 128 bytes of each of the tile's rows.  In LDS a row's 16-byte chunks sit at
@@ -58,9 +59,26 @@ struct Args {
   int nt;                  // store past the caches: C's rows are 16-byte aligned, and C is larger than the Infinity Cache
 };
 
+// Whether sum * sa can leave fp32's range, or its normal numbers, where the product with sb need not: sums are below 2^31.
+__device__ __forceinline__ bool far_scale(float sa) {
+  const float a = fabsf(sa);
+  return (a >= 0x1p97f && a <= 3.402823466e38f) || (a < 0x1p-126f && a > 0.f);
+}
+// sum * sa * sb + bias for any scales: a far sa takes 2^64 from sb or gives it 2^64.  Where sb leaves the range by that the product
+// does too (above, a sum of 1 times 2^97 times 2^64), or is nothing (below 2^31 2^-62 2^-126).
+__device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias) {
+  if (far_scale(sa)) {
+    const bool large = fabsf(sa) >= 1.f;
+    sa *= large ? 0x1p-64f : 0x1p64f;
+    const float far = sb * (large ? 0x1p64f : 0x1p-64f);
+    sb = fabsf(sb) <= 3.402823466e38f ? fminf(fmaxf(far, -3.402823466e38f), 3.402823466e38f) : far;
+  }
+  return fmaf(static_cast<float>(sum) * sa, sb, bias);
+}
+
 template <typename T>
 __device__ __forceinline__ void finish(const Args& g, T* c, int sum, float sa, float sb, float bias) {
-  *c = from_f32<T>(act_fn(fmaf(static_cast<float>(sum) * sa, sb, bias), g.act, g.slope));
+  *c = from_f32<T>(act_fn(scaled(sum, sa, sb, bias), g.act, g.slope));
 }
 
 // 16 codes of a row from k on, zeros past K; any alignment.  Where they end past K the row's last 16 are loaded and moved down, so
@@ -89,9 +107,15 @@ __device__ __forceinline__ void wait_dma() {
   asm volatile("" ::: "memory");
 }
 
+// Waves a SIMD that the registers have to leave room for: 128 of them let two workgroups of 128 x 256 into a compute unit, of which
+// one stores while the other multiplies (10000 x 10677 x 250 into fp32: 126 us a call, with 130 registers 138).  The 16-bit types
+// and the DMA forms of this tile need 132 and more, and spill if held to 128.
+template <typename T, int TM, int TN, bool DMA>
+constexpr int kWavesPerSimd = sizeof(T) == 4 && TM == 128 && TN == 256 && !DMA ? 4 : 1;
+
 // tile TM x TN, waves of WM x WN, K steps of BK bytes, NST LDS stages; DMA: operands are 16-byte aligned
 template <typename T, int TM, int TN, int WM, int WN, int BK, int NST, bool DMA, bool ACT>
-__global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const Args g) {
+__global__ __launch_bounds__(TM / WM * (TN / WN) * 64, (kWavesPerSimd<T, TM, TN, DMA>)) void gemm_i8_kernel(const Args g) {
   constexpr int NWN = TN / WN, NW = TM / WM * NWN, IM = WM / 32, IN = WN / 32, H = BK / 32;
   constexpr int CPR = BK / 16, RP = 64 / CPR;                           // 16-byte chunks a row; a piece: RP rows x BK bytes, one wave access
   constexpr int PA = TM / RP / NW, PB = TN / RP / NW, PIECES = PA + PB, STAGE = (TM + TN) * BK;
@@ -253,7 +277,7 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
   __syncthreads();
   int* cst = reinterpret_cast<int*>(smem) + wave * CST;
   const int first = lane / LPR, rows = g.M - mw - first;
-  const auto block = [&](int i, auto use) {            // use(r, sums): row r of the 32, V sums from column `col` on
+  const auto block = [&](int i, auto rolled, auto use) {      // use(r, sums): row r of the 32, V sums from column `col` on
 #pragma unroll
     for (int j = 0; j < IN; ++j)
 #pragma unroll
@@ -261,7 +285,7 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int UN = ACT ? 1 : 32 / RPP;             // unrolled, the activations' code overflows the instruction cache
+    constexpr int UN = ACT || rolled.value ? 1 : 32 / RPP;      // unrolled, the activations' code overflows the instruction cache
 #pragma unroll UN
     for (int it = 0; it < 32 / RPP; ++it) {
       int v[V];
@@ -277,17 +301,17 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  const auto finish_all = [&](auto store) {
+  const auto finish_all = [&](auto far, auto store) {  // far: some row's scale is, see far_scale
     T* o = static_cast<T*>(g.C) + (mw + first) * g.ldc + n;
     const long long stride = RPP * g.ldc;
 #pragma unroll
     for (int i = 0; i < IM; ++i)
-      block(i, [&](int r, const int* v) {
+      block(i, far, [&](int r, const int* v) {
         const float sa_r = __shfl(sa[i], r);
         float f[V];
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-          f[q] = fmaf(static_cast<float>(v[q]) * sa_r, sb[q], bias[q]);
+          f[q] = far.value ? scaled(v[q], sa_r, sb[q], bias[q]) : fmaf(static_cast<float>(v[q]) * sa_r, sb[q], bias[q]);
           if (ACT) f[q] = act_fn(f[q], g.act, g.slope);
         }
         store(o, f, i * 32 + r - first);
@@ -298,7 +322,7 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
     int* w = g.ws + (static_cast<long long>(z) * g.M + mw + first) * g.N + n;
 #pragma unroll
     for (int i = 0; i < IM; ++i)
-      block(i, [&](int r, const int* v) {
+      block(i, std::false_type{}, [&](int r, const int* v) {
         if (i * 32 + r - first < rows) {
 #pragma unroll
           for (int q = 0; q < V; ++q)
@@ -306,14 +330,18 @@ __global__ __launch_bounds__(TM / WM * (TN / WN) * 64) void gemm_i8_kernel(const
         }
         w += RPP * g.N;
       });
-  } else if (m0 + TM <= g.M && n0 + TN <= g.N) {       // nothing to check
-    if (g.nt) finish_all([](T* o, const float* f, int) { store_vec_nt<T, V>(o, f); });
-    else finish_all([](T* o, const float* f, int) { store_vec<T, V>(o, f, V); });
-  } else {
-    finish_all([&](T* o, const float* f, int r) {
-      if (r < rows && room > 0) store_vec<T, V>(o, f, room);
-    });
+    return;
   }
+  bool far = false;
+#pragma unroll
+  for (int i = 0; i < IM; ++i) far = far || far_scale(sa[i]);
+  const auto store_checked = [&](T* o, const float* f, int r) {
+    if (r < rows && room > 0) store_vec<T, V>(o, f, room);
+  };
+  if (__ballot(far) != 0) finish_all(std::true_type{}, store_checked);
+  else if (m0 + TM > g.M || n0 + TN > g.N) finish_all(std::false_type{}, store_checked);
+  else if (g.nt) finish_all(std::false_type{}, [](T* o, const float* f, int) { store_vec_nt<T, V>(o, f); });
+  else finish_all(std::false_type{}, [](T* o, const float* f, int) { store_vec<T, V>(o, f, V); });
 }
 
 // the splits' sums of one C element, and its epilogue

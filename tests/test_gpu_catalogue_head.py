@@ -1015,3 +1015,35 @@ def test_draw_from_rows_of_millions(n, dtype):
     u = torch.rand(3, generator=g)
     for kw in (dict(), dict(top_p=0.95), dict(top_k=700), dict(top_k=40000, top_p=0.7, min_p=1e-3), dict(min_p=0.01, temperature=0.5)):
         check_draw(l, u, **kw)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 64), (3, 50, 8192), (130, 300, 250), (600, 2100, 64), (2050, 4099, 80), (4096, 4096, 512)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_product_with_scales_over_the_whole_range(M, N, K, dtype):
+    g = torch.Generator(device=DEV).manual_seed(K)
+    a, b = (torch.randint(-128, 128, (n, K), generator=g, device=DEV, dtype=torch.int16).to(torch.int8) for n in (M, N))
+    a[0], b[0] = 0, 0                                      # sums of nothing stay 0 whatever the scales
+    # exponents over all of fp32's, subnormal ones among them; most rows next to each other differ by far
+    sa, sb = (torch.ldexp(torch.rand(n, generator=g, device=DEV) + 0.5, torch.randint(-148, 127, (n,), generator=g, device=DEV)) for n in (M, N))
+    sa[0], sb[N // 2] = 3e38, 3e38
+    sa[M // 2] = 1.7e29
+    sb[1], sb[2] = -1e-30, 0.0
+    bias = torch.randn(N, generator=g, device=DEV)
+    for c, act in ((bias, None), (None, None), (bias, "leaky")):
+        out = ops.gemm_i8(a, sa, b, sb, bias=c, act=act, slope=0.2, out_dtype=dtype).double()
+        exact = a.double() @ b.double().t().contiguous()
+        t = exact * sa.double()[:, None] * sb.double()
+        v = t if c is None else t + c.double()
+        ref = ACTS[act](v)
+        # check_product's roundings; below the normal numbers a rounding is at most half the least number instead (the product
+        # with sb and the sum with the bias are one)
+        fi = torch.finfo(dtype)
+        tol = 1.01 * (2.0 ** -24 * (2 * t.abs() + v.abs() + ref.abs()) + 2.0 ** -149) + (0 if dtype == torch.float32 else fi.eps / 2 * ref.abs() + fi.smallest_normal * fi.eps)
+        edge = fi.max * (1 + fi.eps / 4)                   # the border between the largest number and infinity
+        # what the activation takes is an fp32 number already: 0.2 times an infinity is one, 0.2 times what it stands for need not be
+        room = 2.0 ** 128 * (1 - 2.0 ** -25) - v.abs()
+        small = (ref.abs() + tol < edge) & (room > 2.0 ** 105)
+        past = (ref.abs() - tol >= edge) | (room < -(2.0 ** 105))
+        assert ((out - ref).abs() <= tol)[small].all(), float(((out - ref).abs() - tol)[small].max())
+        assert (out[past] == torch.sign(ref[past]) * INF).all() and not out.isnan().any()
+        assert small.any() and (past.any() or M * N < 1000)
