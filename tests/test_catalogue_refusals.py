@@ -87,3 +87,15 @@ def test_distill_refuses_temperatures_whose_square_leaves_32_bits(temp):
     assert distill(temp=temp) == -1 and distill_bwd(temp=temp) == -1
     for t in (2.0 ** -63, 2.0 ** 63):      # the ends themselves pass this check: the next one refuses the missing workspace
         assert distill(temp=t, ws=None) == -5
+
+
+def test_long_rows_always_ask_for_a_workspace_and_not_for_more_than_a_batch():
+    size = L.lib().sg_sample_rows_workspace_bytes
+    for n in (16385, 1000000, 1 << 20, (1 << 20) + 1, (1 << 30) - 1):
+        for dtype in (0, 1, 2):
+            need = size(1, n, dtype)
+            assert need > 0
+            assert sample(rows=1, n=n, ld=n, dtype=dtype, wsn=need - 1) == -5 and sample(rows=1, n=n, ld=n, dtype=dtype, ws=None, wsn=0) == -5
+    assert size(1, 16384, 0) == 0
+    for rows in (16385, 69878, (1 << 23) - 1):
+        assert size(rows, 20000, 0) == size(16384, 20000, 0) < 1300 << 20

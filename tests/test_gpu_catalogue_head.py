@@ -1047,3 +1047,17 @@ def test_product_with_scales_over_the_whole_range(M, N, K, dtype):
         assert ((out - ref).abs() <= tol)[small].all(), float(((out - ref).abs() - tol)[small].max())
         assert (out[past] == torch.sign(ref[past]) * INF).all() and not out.isnan().any()
         assert small.any() and (past.any() or M * N < 1000)
+
+
+@pytest.mark.parametrize("rows,n,dtype", [(33000, 16390, torch.bfloat16), (16385, 20001, torch.float32)])
+def test_draw_from_more_long_rows_than_one_batch(rows, n, dtype):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    l = (2 * torch.randn(rows, n, generator=g, device=DEV)).to(dtype)
+    u, t, p, m = (torch.rand(rows, generator=g, device=DEV) for _ in range(4))
+    k = torch.randint(0, 3000, (rows,), generator=g, device=DEV)
+    for kw in (dict(), dict(top_p=p), dict(temperature=0.5 + t, top_k=k, top_p=p, min_p=0.01 * m)):
+        ids, prob = ops.sample_rows(l, u, **kw)
+        for lo, hi in ((0, 40), (16370, min(16420, rows)), (rows - 9, rows)):
+            cut = {name: v[lo:hi] for name, v in kw.items()}
+            i, q = ops.sample_rows(l[lo:hi], u[lo:hi], **cut)
+            assert torch.equal(ids[lo:hi], i) and torch.equal(prob[lo:hi], q)
