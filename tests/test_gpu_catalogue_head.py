@@ -1061,3 +1061,76 @@ def test_draw_from_more_long_rows_than_one_batch(rows, n, dtype):
             cut = {name: v[lo:hi] for name, v in kw.items()}
             i, q = ops.sample_rows(l[lo:hi], u[lo:hi], **cut)
             assert torch.equal(ids[lo:hi], i) and torch.equal(prob[lo:hi], q)
+
+
+def test_captured_head_follows_its_inputs_at_every_replay():
+    g = gen(91)
+    items, item_ids = torch.randn(1500, 48, generator=g).to(DEV), torch.randperm(9000, generator=g)[:1500].to(DEV)
+    head = CatalogueHead(items, item_ids=item_ids, norm_weight=torch.ones(48, device=DEV))
+    users, u = torch.empty(9, 48, device=DEV), torch.empty(9, device=DEV)
+    rows, seen = torch.empty(40, dtype=torch.int64, device=DEV), torch.empty(40, dtype=torch.int64, device=DEV)
+
+    def fill(seed):
+        users.copy_(torch.randn(9, 48, generator=gen(seed)))
+        u.copy_(torch.rand(9, generator=gen(seed + 100)))
+        rows.copy_(torch.randint(-1, 10, (40,), generator=gen(seed + 200)))
+        seen.copy_(torch.randint(-1, 9001, (40,), generator=gen(seed + 300)))
+        seen[:9] = item_ids[head.scores(users).argmax(1)]
+        rows[:9] = torch.arange(9, device=DEV)
+
+    def call():
+        return head.draw(users, u, temperature=0.2, top_k=30, top_p=0.95, seen=(rows, seen))
+
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for seed in range(1, 6):
+        fill(seed)
+        want = [v.clone() for v in call()]
+        graph.replay()
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        best = seen[:9]
+        assert (out[0] != best).all() and torch.isin(out[0], item_ids).all()
+
+
+@pytest.mark.parametrize("n", [1682, 16385, 40000, (1 << 20) + 7])
+def test_captured_draws_of_every_length(n):
+    l, u = torch.empty(5, n, device=DEV), torch.empty(5, device=DEV)
+    par = dict(temperature=torch.empty(5, device=DEV), top_k=torch.empty(5, dtype=torch.int64, device=DEV), top_p=torch.empty(5, device=DEV),
+               min_p=torch.empty(5, device=DEV))
+
+    def fill(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        l.normal_(generator=g)
+        for v in (u, par["temperature"], par["top_p"], par["min_p"]):
+            v.uniform_(generator=g)
+        par["top_k"].random_(0, n, generator=g)
+
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.sample_rows(l, u, **par)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for kw in (par, dict(), dict(top_p=0.7)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, kw, ops.sample_rows(l, u, **kw)))
+    for seed in range(1, 5):
+        fill(seed)
+        for graph, kw, out in graphs:
+            want = [v.clone() for v in ops.sample_rows(l, u, **kw)]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
