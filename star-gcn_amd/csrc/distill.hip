@@ -6,8 +6,8 @@
 // An entry whose id lies outside [0, N) or whose score is -inf is no entry.  A row without an entry, or whose student scores
 // are all -inf, has nothing to fit: it adds no loss and its gradient is zero.  An item that is named twice takes both shares.
 //
-// 10000 rows of 10677 bf16 scores: forward 47 us (4.5 TB/s; the chain of one row's entries shows), backward 86 us (5.0 TB/s, a
-// copy of that size reaches 5.3); 64 rows of 1,000,000 fp32: 38 and 87 us (6.7 and 5.9 TB/s).
+// 10000 rows of 10677 bf16 scores: forward 49 us (4.4 TB/s; the chain of one row's entries shows), backward 85 us (5.0 TB/s, a
+// copy of that size reaches 5.3); 64 rows of 1,000,000 fp32: 38 and 87 us (6.8 and 5.9 TB/s).
 //
 // Bound by memory: the forward reads the scores once (running maximum and sum, one exp an element), the backward reads them
 // again and writes the gradient; the K entries of a row are noise next to its N scores.  Long rows of small batches are split

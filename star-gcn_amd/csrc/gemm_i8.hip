@@ -18,8 +18,8 @@
 //
 // What bounds it, measured on an MI355X.  8192 x 8192 x 4096 into bf16: 229 us, 2.4 POP/s, for quantised normal rows, 281 us for
 // uniformly random codes, 181 us for zeros: the chip's power sets the clock (1.7 GHz in the counters' runs), the matrix units are
-// busy 72 % of the cycles.  A K-short product (10000 x 10677 x 256 into fp32) is bound by its stores: 106 us, 4 TB/s against 6.6
-// TB/s of a fill of the same buffer; K = 250, through registers, takes 115.  One row against 10677: 4.5 us of a call of 12.
+// busy 72 % of the cycles.  A K-short product (10000 x 10677 x 256 into fp32) is bound by its stores: 106 to 112 us, 4 TB/s
+// against 6.6 TB/s of a fill of the same buffer; K = 250, through registers, takes 115 to 118.  One row against 10677: 4.5 us of a call of 12.
 #include "rows_shared.hpp"
 
 #include <algorithm>
@@ -36,7 +36,7 @@ using f16x3::act_fn;
 using f16x3::glb_void;
 using f16x3::lds_void;
 
-constexpr int GROUP = 8;                   // columns of tiles in a band; 4, 16 and whole rows of tiles were 1 to 2 % slower
+constexpr int GROUP = 8;                   // columns of tiles in a band; 4 and 16 run from 1 % faster to 4 % slower
 
 // slot of 16-byte chunk c of a row in LDS: c ^ swizzle(row)
 template <int BK>

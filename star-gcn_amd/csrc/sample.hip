@@ -19,8 +19,9 @@
 //
 // Rows of up to 16384 items: one workgroup a row, the row in LDS.  Longer rows are cut into pieces, five launches: maximum;
 // histogram; the limits' bins; weight by index of what is surely kept, and the list of the limits' candidates; limits and draw.
-// A list of more than 8192 candidates (many equal scores) is replaced by passes over the row.  64 rows of 1,000,000 fp32 scores,
-// top-p: 38 us for the maximum (6.7 TB/s), 61 for the histogram (bound by the 64-bit arithmetic: 24 operations an item), 10, 52 and
+// A list of more than 8192 candidates (many equal scores, or a spread that is small beside T) is replaced by passes of one workgroup
+// over the row: 64 rows of 1,000,000 scores of deviation 0.5 T then take 1.6 ms.  64 rows of 1,000,000 fp32 scores,
+// top-p: 37 us for the maximum (6.9 TB/s), 61 for the histogram (bound by the 64-bit arithmetic: 24 operations an item), 10, 52 and
 // 12 for the rest.
 #include "rows_shared.hpp"
 
@@ -431,7 +432,7 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 // ---- one workgroup a row, the row in LDS ------------------------------------------------------------------------------------
 // In registers the compiler keeps what one pass derives from a score for the next, for every score, and spills (69 us instead of
 // 43 for 512 rows of 10677).  What bounds a row is 64-bit arithmetic on one compute unit, two passes of ~24 operations an item,
-// not its barriers (eleven instead of twenty: 16.4 -> 15.9 us for 10677 items).
+// not its barriers (eleven instead of twenty saved half a microsecond): 14.5 us for 10677 items.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(const SampleArgs g) {
   __shared__ Shared<u64> sh;
