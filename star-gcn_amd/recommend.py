@@ -19,7 +19,6 @@ from . import ops
 def _mask_pairs(scores, rows, items):
     """scores[rows[i], items[i]] = -inf; pairs outside the scores are passed over.  A minimum with +inf changes nothing, so this
     needs neither a look at the indices on the host nor a list of the valid ones, and can be captured."""
-    L.require_current_gpu(scores, rows, items)
     if rows.is_floating_point() or items.is_floating_point() or torch.bool in (rows.dtype, items.dtype):
         raise L.StarGCNError("CatalogueHead: seen is a pair of index tensors, got %s and %s" % (rows.dtype, items.dtype))
     try:
@@ -49,7 +48,7 @@ class CatalogueHead(object):
         self.codes, self.scale = ops.quantize_rows(item_rows.detach())
         self.bias, self.norm_weight, self.eps = bias, norm_weight, eps
         self.items = self.codes.shape[0]
-        self.item_ids = item_ids
+        self.item_ids = None if item_ids is None else item_ids.clone()
         if item_ids is not None:
             L.require_current_gpu(item_ids)
             if item_ids.dtype not in (torch.int32, torch.int64) or item_ids.shape != (self.items,):
@@ -79,14 +78,15 @@ class CatalogueHead(object):
         return torch.where(self._sorted_ids[at] == ids, self._sorted_rows[at], torch.full_like(at, -1))
 
     def draw(self, user_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, residual=None, seen=None):
-        """One item a user row -> (ids int32, prob fp32), see ops.sample_rows.  seen: (rows of user_rows, item
-        ids) index pair of what is not to be drawn, e.g. the items that a user has rated (a pair outside the scores, such as
+        """One item a user row -> (ids int32 or of item_ids' type, prob fp32), see ops.sample_rows.  seen: (rows of
+        user_rows, item ids) index pair of what is not to be drawn, e.g. the items that a user has rated (a pair outside the scores, such as
         padding of -1 or an item that is not in the catalogue, names nothing); a user who has seen everything gets id -1."""
         s = self.scores(user_rows, residual=residual)
         if seen is not None:
-            L.require_current_gpu(*seen)
-            _mask_pairs(s, seen[0], self._rows_of(seen[1]))
+            rows, items = (t.to(s.device) for t in seen)
+            _mask_pairs(s, rows, self._rows_of(items))
         ids, prob = ops.sample_rows(s, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        if self.item_ids is not None and self.items:
-            ids = torch.where(ids >= 0, self.item_ids[ids.clamp(min=0).long()], torch.full_like(self.item_ids[:1], -1))
+        if self.item_ids is not None:
+            named = self.item_ids[ids.clamp(min=0).long()] if self.items else ids.to(self.item_ids.dtype)
+            ids = torch.where(ids >= 0, named, torch.full_like(named, -1))
         return ids, prob

@@ -792,8 +792,8 @@ def test_seen_pairs_outside_the_scores_name_nothing():
             want, got = ops.sample_rows(masked, u, **kw), head.draw(users, u, seen=seen, **kw)
             assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
     best = s.argmax(1)
-    ids, _ = head.draw(users, u, top_k=1, seen=(torch.arange(5, device=DEV).int(), best.int()))
-    assert (ids != best).all()
+    second, _ = head.draw(users, u, top_k=1, seen=(torch.arange(5, device=DEV).int(), best.int()))
+    assert (second != best).all()
     every = (torch.arange(5, device=DEV)[:, None], torch.arange(200, device=DEV))      # every pair
     ids, prob = head.draw(users, u, seen=every)
     assert (ids == -1).all() and (prob == 0).all()
@@ -801,7 +801,10 @@ def test_seen_pairs_outside_the_scores_name_nothing():
     lost[0, 1] = math.nan                                  # scores of NaN stay what is never drawn
     ids, prob = head.draw(lost, u, seen=(i64([-1, 0]), i64([-1, 2])))
     assert ids[0] == -1 and (ids[1:] >= 0).all()
-    for bad in ((best, best[:3]), (best, best.float()), (best > 0, best), (best.cpu(), best)):
+    rows = torch.arange(5)
+    on_host, _ = head.draw(users, u, top_k=1, seen=(rows, best.cpu()))
+    assert torch.equal(on_host, second)
+    for bad in ((best, best[:3]), (best, best.float()), (best > 0, best)):
         with pytest.raises(L.StarGCNError):
             head.draw(users, u, seen=bad)
 
@@ -854,7 +857,7 @@ def test_item_ids_are_checked():
     got, _ = CatalogueHead(x, item_ids=ids).draw(x, torch.rand(4, device=DEV), top_k=1, seen=(torch.zeros(1, dtype=torch.int64, device=DEV), ids[1:2]))
     assert all(v in ids.tolist() for v in got.tolist()) and got[0] != 1 << 40
     none, prob = CatalogueHead(x[:0], item_ids=ids[:0]).draw(x, torch.rand(4, device=DEV), seen=(ids[:1], ids[:1]))
-    assert none.tolist() == [-1] * 4
+    assert none.tolist() == [-1] * 4 and none.dtype == torch.int64
     small, _ = CatalogueHead(x, item_ids=torch.tensor([9, 8, 7, 6], dtype=torch.int32, device=DEV)).draw(x, torch.rand(4, device=DEV))
     assert small.dtype == torch.int32
     for bad in (ids[:3], ids.cpu(), ids.float(), ids[None], torch.tensor([1, 2, 2, 3], device=DEV), torch.tensor([1, 2, -2, 3], device=DEV)):
