@@ -534,8 +534,8 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     min_p times as likely as the best (0: all).  Each setting is a number, or a tensor with one a row.  -> (ids int32, prob
     fp32: the drawn item's probability among the kept ones).  Equal scores rank by index; scores of -inf and NaN are never
     drawn; a row of nothing else gives id -1, prob 0.  The same inputs draw the same items in every run.  Weights are whole numbers
-    of 2^-51 of the best item's (2^-43 for 2^19 to 2^20 items): what a row's items gain or lose by it is at most 2^-24 of the best item's weight up to
-    2^28 items, 2^-22 at 2^30, and an item below half a unit is never drawn."""
+    of 2^-51 of the best item's (2^-43 at a million items, which are summed in 64 bits): what a row's items gain or lose by it is at
+    most 2^-24 of the best item's weight up to 2^28 items, 2^-22 at 2^30, and an item below half a unit is never drawn."""
     L.require_current_gpu(logits, u)
     dt = _dtype_id(logits, "sample_rows")
     logits, ld = _rows(logits, "sample_rows")
